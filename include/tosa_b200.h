@@ -4,7 +4,9 @@
  * (and MATMUL_T, TRANSPOSE_CONV2D, CONV3D) with their zero points, bias and
  * acc_type, fused with the RESCALE (and
  * CLAMP) that follows them, plus AVG_POOL2D / MAX_POOL2D and the glue ops the
- * quantized graphs need (standalone RESCALE, CLAMP, ADD).
+ * quantized graphs need (standalone RESCALE, CLAMP, ADD); and, for serving the
+ * transformer blocks whose MATMULs it runs, attention over packed prompts and a
+ * paged key-value cache with the attention that reads it.
  *
  * C ABI: plain pointers and sizes, no C++ types, no exceptions across the
  * boundary. Every entry point returns a tb_status; on failure the thread's
@@ -66,7 +68,8 @@ typedef enum tb_status {
     TB_ERR_CUDA = 64,            /* a CUDA call failed */
     TB_ERR_TIMEOUT = 65,         /* a bounded device wait gave up */
     TB_ERR_INVALID_ARGUMENT = 66,/* null pointer, bad handle */
-    TB_ERR_NOT_ACCELERATED = 67  /* valid TOSA this backend does not run (caller keeps its own path) */
+    TB_ERR_NOT_ACCELERATED = 67, /* valid TOSA this backend does not run (caller keeps its own path) */
+    TB_ERR_OUT_OF_PAGES = 68     /* a key-value cache has too few free pages */
 } tb_status;
 
 /* DType codes: the serialized TOSA DType enum (schema/tosa.fbs:26-46). */
@@ -92,7 +95,9 @@ TB_API const char *tb_last_error(void);
 /* Wait for `stream`, then read and clear the context's device error word;
  * returns TB_ERR_GRAPH if a kernel hit a RESCALE/apply_scale range error
  * (src/ops/quant.rs:18-25, src/ops/type_conv.rs:183-186), TB_ERR_TIMEOUT if a
- * bounded wait gave up. */
+ * bounded wait gave up, TB_ERR_INVALID_ARGUMENT if an attention or cache
+ * operator met an index out of range in a device array, TB_ERR_OUT_OF_PAGES if
+ * a cache ran out of pages. */
 TB_API tb_status tb_synchronize(tb_context *ctx, void *stream);
 TB_API tb_status tb_malloc(tb_context *ctx, size_t bytes, void **dptr);
 TB_API tb_status tb_free(tb_context *ctx, void *dptr);
@@ -300,6 +305,112 @@ TB_API tb_status tb_avg_pool2d(tb_context *ctx, const tb_pool2d_desc *desc, cons
                                void *stream);
 TB_API tb_status tb_max_pool2d(tb_context *ctx, const tb_pool2d_desc *desc, const void *input, void *out,
                                void *stream);
+
+/* ---- attention over packed prompts ------------------------------------------
+ * No counterpart in the reference; it joins the two MATMULs of a transformer
+ * block's attention through the softmax between them. `batch` sequences lie one
+ * behind the other in q / out (total_q rows) and in k / v (total_k rows):
+ * sequence b has the rows cu_q[b] .. cu_q[b+1]-1 and the keys cu_k[b] ..
+ * cu_k[b+1]-1 (DEVICE arrays of batch+1 int32 offsets, non-decreasing, within
+ * 0 .. total). With i counted within the rows and j within the keys of a
+ * sequence of lq rows and lk keys, query head h and key head h / (q_heads /
+ * kv_heads):
+ *   out[i,h] = sum_j w_j v[j] / sum_j w_j,  w_j = exp(scale * q[i,h].k[j]),
+ *   lse[h][i] = log sum_j w_j  (FP32, [q_heads][total_q]; lse may be NULL),
+ * over every j, or with `causal` over j <= i + lk - lq (the last row sees every
+ * key). A row that sees no key gives out 0 and lse -inf. Keys that a row does
+ * not see have no part in it, whatever they hold. Products are of f16 / bf16
+ * operands with FP32 sums; the weights are rounded to the operands' type for
+ * the second product and are summed in FP32 before that rounding.
+ * head_dim is a multiple of 16 up to 128 and q_heads a multiple of kv_heads.
+ * Strides are elements from one token to the next and from one head to the next
+ * (head_dim elements of a head are contiguous); strides are multiples of 8 and
+ * pointers 16-byte aligned, so q, k and v may be parts of one projection's rows.
+ * Asynchronous on `stream`; offsets out of range leave the sequence's rows
+ * unwritten and are reported by the next tb_synchronize. */
+typedef struct tb_attention_desc {
+    int32_t dtype;            /* TB_DT_BF16 / TB_DT_FP16: q, k, v and out */
+    int32_t batch;
+    int32_t q_heads, kv_heads, head_dim;
+    int32_t causal;
+    float scale;              /* positive */
+    int64_t total_q, total_k;
+    int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2]; /* token, head */
+} tb_attention_desc;
+TB_API tb_status tb_attention(tb_context *ctx, const tb_attention_desc *desc, const void *q, const void *k,
+                              const void *v, const int32_t *cu_q, const int32_t *cu_k, void *out, float *lse,
+                              void *stream);
+
+/* ---- paged key-value cache ---------------------------------------------------
+ * No counterpart in the reference. Keys and values of up to max_seqs sequences
+ * ("slots") live in pages of page_size tokens; every buffer is the caller's
+ * device memory and stays in place for the life of the handle:
+ *   k_pages, v_pages  [layers][num_pages][kv_heads][page_size][head_dim], f16 / bf16
+ *   page_table        int32 [max_seqs][max_pages]: entry j of a slot is the page of its
+ *                     tokens j*page_size ..; -1 past its last page
+ *   lengths           int32 [max_seqs]: tokens of each slot (0: the slot is empty)
+ *   refs              int32 [num_pages]: slots that hold the page; 0 is free
+ * A page that is not full belongs to one slot; full pages may be shared. A cache
+ * starts with page_table -1, lengths 0 and refs 0. Slots, counts, offsets and
+ * page ids passed below are DEVICE int32 arrays, so a step needs no host copy
+ * and can be captured in a CUDA graph. Calls on one cache must not overlap on
+ * the GPU (they share its state and workspace): use one stream, or order them.
+ * Index arrays are checked on the device: a bad slot, page, length or a page
+ * shortage leaves the state unchanged and is reported by the next
+ * tb_synchronize (TB_ERR_INVALID_ARGUMENT / TB_ERR_OUT_OF_PAGES). */
+typedef struct tb_cache_desc {
+    int32_t dtype;            /* TB_DT_BF16 / TB_DT_FP16 */
+    int32_t layers, kv_heads, head_dim; /* head_dim: a multiple of 16 up to 128 */
+    int32_t page_size;        /* a multiple of 8 */
+    int32_t num_pages, max_seqs, max_pages;
+} tb_cache_desc;
+typedef struct tb_cache_buffers {
+    void *k_pages, *v_pages;  /* 16-byte aligned */
+    int32_t *page_table, *lengths, *refs;
+} tb_cache_buffers;
+typedef struct tb_cache tb_cache;
+TB_API tb_status tb_cache_create(tb_context *ctx, const tb_cache_desc *desc, const tb_cache_buffers *buffers,
+                                 tb_cache **out);
+TB_API void tb_cache_destroy(tb_cache *cache);
+/* Grow slots[i] by counts[i] tokens (counts NULL: one each): lengths go up and
+ * the pages that are needed are taken, lowest free page first, in the order of
+ * i. Slots are distinct. Their contents are written by tb_cache_write. */
+TB_API tb_status tb_cache_reserve(tb_cache *cache, const int32_t *slots, const int32_t *counts, int32_t n,
+                                  void *stream);
+/* Write the last tokens of n slots in one layer: the rows offsets[i] ..
+ * offsets[i+1]-1 of k and v ([total][kv_heads][head_dim], strides token and head)
+ * are the keys and values of the last offsets[i+1]-offsets[i] tokens of slots[i]. */
+TB_API tb_status tb_cache_write(tb_cache *cache, int32_t layer, const int32_t *slots, const int32_t *offsets,
+                                int32_t n, int64_t total, const void *k, int64_t k_token_stride,
+                                int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride,
+                                void *stream);
+/* Attention of one new token each of n slots over all its tokens in the cache
+ * (tb_attention's formula with one row a sequence; the token's own key has been
+ * written): q and out [n][q_heads][head_dim] with strides sequence and head,
+ * lse FP32 [n][q_heads] or NULL. An empty slot gives out 0 and lse -inf. */
+TB_API tb_status tb_cache_attend(tb_cache *cache, int32_t layer, const int32_t *slots, int32_t n, int32_t q_heads,
+                                 float scale, const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
+                                 int64_t out_seq_stride, int64_t out_head_stride, float *lse, void *stream);
+/* Make children[i] a copy of parents[i]: full pages are shared, the tokens of a
+ * last page that is not full are copied (every layer) to the lowest free page,
+ * in the order of i. What a child held before is freed first. Children are
+ * distinct and none is a parent in the same call. */
+TB_API tb_status tb_cache_fork(tb_cache *cache, const int32_t *parents, const int32_t *children, int32_t n,
+                               void *stream);
+/* Empty n distinct slots; pages that no slot holds any more become free. */
+TB_API tb_status tb_cache_free(tb_cache *cache, const int32_t *slots, int32_t n, void *stream);
+/* Copy the contents of the pages src[i] to the pages dst[i], in every layer
+ * (pages only: page_table and refs are not touched). No dst is also a src or
+ * occurs twice. */
+TB_API tb_status tb_cache_copy_pages(tb_cache *cache, const int32_t *src, const int32_t *dst, int32_t n,
+                                     void *stream);
+/* Move the pages in use to the front: with L pages in use, the k-th page in use
+ * at L or above goes to the k-th free page below L (contents of every layer,
+ * page_table and refs). With page_table_out / refs_out (both or neither) the new
+ * table and counts are written there and the cache's own stay as they were; the
+ * old places of moved pages keep their contents, so readers of the old table
+ * stay right until a page is taken again. */
+TB_API tb_status tb_cache_compact(tb_cache *cache, int32_t *page_table_out, int32_t *refs_out, void *stream);
 
 /* ---- graph runner ----------------------------------------------------------
  * Runs a serialized TOSA graph (.tosa flatbuffer) on the device: the

@@ -24,8 +24,10 @@ STATUS_NAMES = {
     0: "OK", 1: "Deserialize", 2: "UnsupportedOp", 3: "TensorNotFound", 4: "DTypeMismatch",
     5: "ShapeMismatch", 6: "Broadcast", 7: "GraphError", 8: "ControlFlow", 9: "Io",
     64: "Cuda", 65: "Timeout", 66: "InvalidArgument", 67: "NotAccelerated",
+    68: "OutOfPages",
 }
-TB_ERR_NOT_ACCELERATED = 67
+TB_ERR_DTYPE_MISMATCH, TB_ERR_SHAPE_MISMATCH = 4, 5
+TB_ERR_INVALID_ARGUMENT, TB_ERR_NOT_ACCELERATED, TB_ERR_OUT_OF_PAGES = 66, 67, 68
 
 
 class TbError(RuntimeError):
@@ -73,6 +75,21 @@ class Pool2dDesc(ctypes.Structure):
                 ("kernel", ctypes.c_int32 * 2), ("stride", ctypes.c_int32 * 2), ("pad", ctypes.c_int32 * 4),
                 ("dtype", ctypes.c_int32), ("acc_dtype", ctypes.c_int32), ("input_zp", ctypes.c_int32),
                 ("output_zp", ctypes.c_int32), ("nan_mode", ctypes.c_int32)]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "batch", "q_heads", "kv_heads", "head_dim", "causal")] + \
+               [("scale", ctypes.c_float), ("total_q", ctypes.c_int64), ("total_k", ctypes.c_int64)] + \
+               [(n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+
+
+class CacheDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "layers", "kv_heads", "head_dim", "page_size", "num_pages",
+                                              "max_seqs", "max_pages")]
+
+
+class CacheBuffers(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_pages", "v_pages", "page_table", "lengths", "refs")]
 
 
 class TensorInfo(ctypes.Structure):
@@ -140,6 +157,16 @@ SIGNATURES = [
     ("tb_add", _I, [_V, _I, _V, _V, _L, _V, _V]),
     ("tb_avg_pool2d", _I, [_V, _P(Pool2dDesc), _V, _V, _V]),
     ("tb_max_pool2d", _I, [_V, _P(Pool2dDesc), _V, _V, _V]),
+    ("tb_attention", _I, [_V, _P(AttentionDesc), _V, _V, _V, _V, _V, _V, _V, _V]),
+    ("tb_cache_create", _I, [_V, _P(CacheDesc), _P(CacheBuffers), _P(_V)]),
+    ("tb_cache_destroy", None, [_V]),
+    ("tb_cache_reserve", _I, [_V, _V, _V, _I, _V]),
+    ("tb_cache_write", _I, [_V, _I, _V, _V, _I, _L, _V, _L, _L, _V, _L, _L, _V]),
+    ("tb_cache_attend", _I, [_V, _I, _V, _I, _I, ctypes.c_float, _V, _L, _L, _V, _L, _L, _V, _V]),
+    ("tb_cache_fork", _I, [_V, _V, _V, _I, _V]),
+    ("tb_cache_free", _I, [_V, _V, _I, _V]),
+    ("tb_cache_copy_pages", _I, [_V, _V, _V, _I, _V]),
+    ("tb_cache_compact", _I, [_V, _V, _V, _V]),
     ("tb_graph_load", _I, [_V, _V, ctypes.c_size_t, ctypes.c_uint32, _P(_V)]),
     ("tb_graph_destroy", None, [_V]),
     ("tb_graph_num_inputs", _I, [_V]),

@@ -452,6 +452,10 @@ TB_API tb_status tb_synchronize(tb_context* ctx, void* stream) {
         if (word & DEV_ERR_TIMEOUT) return fail(TB_ERR_TIMEOUT, "a device wait timed out (error word 0x%x)", word);
         if (word & DEV_ERR_SCALE)
             return fail(TB_ERR_GRAPH, "apply_scale: value out of range for the shift, or result exceeds int32");
+        if (word & DEV_ERR_INDEX)
+            return fail(TB_ERR_INVALID_ARGUMENT, "attention or cache: an offset, slot, page or length on the device is "
+                                                 "out of range");
+        if (word & DEV_ERR_PAGES) return fail(TB_ERR_OUT_OF_PAGES, "cache: not enough free pages");
         return fail(TB_ERR_GRAPH, "device error word 0x%x", word);
     }
     return TB_OK;

@@ -18,6 +18,8 @@ enum : uint32_t {
     DEV_ERR_SCALE = 1u,    // apply_scale range / int32 overflow (Error::GraphError)
     DEV_ERR_TIMEOUT = 2u,  // a bounded wait gave up
     DEV_ERR_INTERNAL = 4u,
+    DEV_ERR_INDEX = 8u,    // an offset, slot, page id or length in device memory is out of range
+    DEV_ERR_PAGES = 16u,   // the cache has too few free pages
 };
 
 // Rounding modes (schema RoundingMode enum).
