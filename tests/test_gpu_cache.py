@@ -203,32 +203,32 @@ def test_attend_bad_indices_are_reported(ctx):
     lens = [30, 40, 50]
     c, k, v = _filled(ctx, 6, "bf16", lens, 1, 64, 16)
     q = torch.randn(3, 2, 64, device="cuda").bfloat16()
-    want, _ = c.attend(0, _ints([0, 1, 2]), q)
-    ctx.synchronize()
     keep = c.page_table.clone(), c.lengths.clone()
 
-    def refused(slots):
-        out, _ = c.attend(0, _ints(slots), q)
+    def refused(slots, *right):
+        """The call is refused; the rows of `right` are right all the same."""
+        out, lse = c.attend(0, _ints(slots), q)
         with pytest.raises(L.TbError) as e:
             ctx.synchronize()
         assert e.value.kind == "InvalidArgument"
+        right = list(right)
+        _check("bf16", q[right], k, v, lens, [slots[r] for r in right], np.float32(0.125), out[right], lse[right])
         c.page_table.copy_(keep[0])
         c.lengths.copy_(keep[1])
-        return out
 
-    assert torch.equal(refused([0, 3, 2])[[0, 2]], want[[0, 2]])
-    assert torch.equal(refused([-1, 1, 2])[1:], want[1:])
+    refused([0, 3, 2], 0, 2)
+    refused([-1, 1, 2], 1, 2)
     c.page_table[1, 1] = 1000000
-    assert torch.equal(refused([0, 1, 2])[[0, 2]], want[[0, 2]])
+    refused([0, 1, 2], 0, 2)
     c.page_table[1, 2] = -7
-    assert torch.equal(refused([0, 1, 2])[[0, 2]], want[[0, 2]])
+    refused([0, 1, 2], 0, 2)
     c.lengths[2] = 1 << 30
-    assert torch.equal(refused([0, 1, 2])[:2], want[:2])
+    refused([0, 1, 2], 0, 1)
     c.lengths[0] = -1
-    assert torch.equal(refused([0, 1, 2])[1:], want[1:])
-    got, _ = c.attend(0, _ints([0, 1, 2]), q)
+    refused([0, 1, 2], 1, 2)
+    out, lse = c.attend(0, _ints([0, 1, 2]), q)
     ctx.synchronize()
-    assert torch.equal(got, want)
+    _check("bf16", q, k, v, lens, [0, 1, 2], np.float32(0.125), out, lse)
 
 
 def test_a_cache_beyond_32_bit_offsets(ctx):

@@ -561,6 +561,11 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
     c->job_src = c->remap + d->num_pages;
     c->job_dst = c->job_src + d->num_pages;
     c->job_rows = c->job_dst + d->num_pages;
+    const tb_status st = decode_create(c);
+    if (st != TB_OK) {
+        tb_cache_destroy(c);
+        return st;
+    }
     *out = c;
     return TB_OK;
 }
@@ -568,6 +573,7 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
 TB_API void tb_cache_destroy(tb_cache* c) {
     if (!c) return;
     if (c->blob) cudaFree(c->blob);
+    decode_destroy(c);
     delete c;
 }
 

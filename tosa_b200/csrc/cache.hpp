@@ -1,7 +1,15 @@
 // The paged key-value cache's handle, shared by its translation units.
 #pragma once
 
+#include <vector>
+
 #include "internal.hpp"
+
+namespace tb {
+// The attention kernel's maps and workspace (decode.cu), made with the cache.
+tb_status decode_create(tb_cache* c);
+void decode_destroy(tb_cache* c);
+}  // namespace tb
 
 struct tb_cache {
     tb_context* ctx = nullptr;
@@ -17,4 +25,10 @@ struct tb_cache {
     int32_t* job_dst = nullptr;  // ... to this page ...
     int32_t* job_rows = nullptr; // ... this many tokens
     void* blob = nullptr;
+    // Attention of one new token: what a CTA leaves of a unit that others share (decode.cu)
+    float* part_o = nullptr;     // [2 * CTAs][16][head_dim]
+    float2* part_ml = nullptr;   // [2 * CTAs][16]
+    uint32_t* arrived = nullptr; // [CTAs] zero between calls
+    int decode_ctas = 0;
+    std::vector<CUtensorMap> k_map, v_map;  // of each layer
 };
