@@ -335,7 +335,8 @@ typedef struct tb_attention_desc {
     int32_t causal;
     float scale;              /* positive */
     int64_t total_q, total_k;
-    int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2]; /* token, head */
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
 } tb_attention_desc;
 TB_API tb_status tb_attention(tb_context *ctx, const tb_attention_desc *desc, const void *q, const void *k,
                               const void *v, const int32_t *cu_q, const int32_t *cu_k, void *out, float *lse,

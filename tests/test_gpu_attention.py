@@ -259,9 +259,10 @@ def test_offsets_out_of_range_are_reported(ctx, cu_q, cu_k):
 
 def _desc(**kw):
     d = dict(dtype=L.DT_BF16, batch=1, q_heads=2, kv_heads=1, head_dim=64, causal=1, scale=0.125, total_q=4, total_k=4,
-             q_stride=(128, 64), k_stride=(64, 64), v_stride=(64, 64), out_stride=(128, 64))
+             q_token_stride=128, q_head_stride=64, k_token_stride=64, k_head_stride=64, v_token_stride=64, v_head_stride=64,
+             out_token_stride=128, out_head_stride=64)
     d.update(kw)
-    return L.AttentionDesc(**{n: (ctypes.c_int64 * 2)(*x) if n.endswith("stride") else x for n, x in d.items()})
+    return L.AttentionDesc(**d)
 
 
 @pytest.mark.parametrize("change,kind", [
@@ -269,8 +270,8 @@ def _desc(**kw):
     (dict(head_dim=136), "NotAccelerated"), (dict(head_dim=24), "NotAccelerated"), (dict(head_dim=0), "NotAccelerated"),
     (dict(scale=0.0), "InvalidArgument"), (dict(scale=-1.0), "InvalidArgument"), (dict(scale=math.nan), "InvalidArgument"),
     (dict(scale=math.inf), "InvalidArgument"), (dict(batch=-1), "ShapeMismatch"), (dict(total_q=-1), "ShapeMismatch"),
-    (dict(total_k=1 << 31), "NotAccelerated"), (dict(q_stride=(130, 64)), "InvalidArgument"),
-    (dict(v_stride=(-64, 64)), "ShapeMismatch"), (dict(k_stride=(64, 4)), "InvalidArgument"),
+    (dict(total_k=1 << 31), "NotAccelerated"), (dict(q_token_stride=130), "InvalidArgument"),
+    (dict(v_token_stride=-64), "ShapeMismatch"), (dict(k_head_stride=4), "InvalidArgument"),
 ])
 def test_refusals(ctx, change, kind):
     t = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")

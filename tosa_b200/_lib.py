@@ -80,7 +80,7 @@ class Pool2dDesc(ctypes.Structure):
 class AttentionDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "batch", "q_heads", "kv_heads", "head_dim", "causal")] + \
                [("scale", ctypes.c_float), ("total_q", ctypes.c_int64), ("total_k", ctypes.c_int64)] + \
-               [(n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+               [(f"{n}_{s}_stride", ctypes.c_int64) for n in ("q", "k", "v", "out") for s in ("token", "head")]
 
 
 class CacheDesc(ctypes.Structure):

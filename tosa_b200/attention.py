@@ -20,13 +20,15 @@ shapes, strides, alignment) raises TbError at the call.
 from __future__ import annotations
 
 import ctypes
-import math
+
 
 import torch
 
 from . import _lib as L
 
 _DTYPES = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_FP16}
+_INT32 = torch.int32
+_F32 = torch.float32
 
 
 def _refuse(status: int, message: str):
@@ -40,33 +42,53 @@ def _dtype(t, op):
     return code
 
 
+# Small calls take a few microseconds on the GPU, so the checks that every call makes are written to be
+# quick: one look at each tensor, and the reason of a refusal is worked out only when there is one.
+
 def _heads(op, name, t, dtype, device, rows=None, heads=None, dim=None):
-    """Checks a [rows, heads, head_dim] tensor whose heads are contiguous; returns its token and head strides."""
-    if t.dtype != dtype:
-        _refuse(L.TB_ERR_DTYPE_MISMATCH, f"{op}: {name} is {t.dtype}, not {dtype}")
-    if t.device != device:
-        _refuse(L.TB_ERR_INVALID_ARGUMENT, f"{op}: {name} is on {t.device}, not on {device}")
-    if t.dim() != 3 or any(w is not None and w != g for w, g in zip((rows, heads, dim), t.shape)):
+    """Checks a [rows, heads, head_dim] tensor on device number `device` whose heads are contiguous (None: any
+    number); returns its token and head strides."""
+    try:
+        n, h, d = t.shape
+        token, head, last = t.stride()
+    except ValueError:
+        n = None
+    if (n is None or t.dtype is not dtype or t.get_device() != device or last != 1 or (rows is not None and n != rows)
+            or (heads is not None and h != heads) or (dim is not None and d != dim)):
+        if t.dtype is not dtype:
+            _refuse(L.TB_ERR_DTYPE_MISMATCH, f"{op}: {name} is {t.dtype}, not {dtype}")
+        if t.get_device() != device:
+            _refuse(L.TB_ERR_INVALID_ARGUMENT, f"{op}: {name} is on {t.device}, not on device {device}")
+        if t.dim() == 3 and t.stride(2) != 1:
+            _refuse(L.TB_ERR_SHAPE_MISMATCH, f"{op}: the last dimension of {name} must be contiguous")
         _refuse(L.TB_ERR_SHAPE_MISMATCH, f"{op}: {name} has shape {tuple(t.shape)}")
-    if t.stride(2) != 1:
-        _refuse(L.TB_ERR_SHAPE_MISMATCH, f"{op}: the last dimension of {name} must be contiguous")
     # the stride of a dimension of one element says nothing
-    token, head = t.stride(0), t.stride(1)
-    return (token if t.shape[0] > 1 else t.shape[1] * t.shape[2]), (head if t.shape[1] > 1 else t.shape[2])
+    return (token if n > 1 else h * d), (head if h > 1 else d)
 
 
 def _index(op, name, t, n, device):
-    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+    """Checks a contiguous int32 vector of n (None: any number) on the device; returns its length."""
+    if t.dtype is not _INT32 or t.dim() != 1 or (n is not None and t.numel() != n) or not t.is_contiguous():
         _refuse(L.TB_ERR_SHAPE_MISMATCH, f"{op}: {name} must be a contiguous int32 vector" + ("" if n is None else f" of {n}"))
-    if t.device != device:
-        _refuse(L.TB_ERR_INVALID_ARGUMENT, f"{op}: {name} is on {t.device}, not on {device}")
+    if t.get_device() != device:
+        _refuse(L.TB_ERR_INVALID_ARGUMENT, f"{op}: {name} is on {t.device}, not on device {device}")
+    return t.numel()
 
 
-def _on(stream, tensors):
+def _sums(op, lse, rows, columns, device):
+    if lse.dtype is not _F32 or tuple(lse.shape) != (rows, columns) or not lse.is_contiguous() or lse.get_device() != device:
+        _refuse(L.TB_ERR_SHAPE_MISMATCH, f"{op}: lse must be contiguous float32 of ({rows}, {columns})")
+
+
+# The current stream's handle; torch.cuda.current_stream() makes a stream object first, a few microseconds.
+_current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _on(stream, device, *tensors):
     """The raw stream a call runs on. Tensors that meet another stream than the current one are held
     for it by the allocator until the call's work is done."""
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        return _current(device)
     for t in tensors:
         if t is not None:
             t.record_stream(stream)
@@ -78,30 +100,30 @@ def attention(ctx, q, k, v, cu_q, cu_k, *, causal=True, scale=None, out=None, ls
     [total_k, kv_heads, head_dim], cu_q and cu_k int32 offsets of batch + 1. Returns (out, lse), out
     like q, lse float32 [q_heads, total_q]. `scale` defaults to 1 / sqrt(head_dim)."""
     op = "attention"
-    code = _dtype(q.dtype, op)
-    device = q.device
-    sq = _heads(op, "q", q, q.dtype, device)
+    dtype = q.dtype
+    code = _dtype(dtype, op)
+    device = q.get_device()
+    q_token, q_head = _heads(op, "q", q, dtype, device)
     rows, heads, dim = q.shape
-    sk = _heads(op, "k", k, q.dtype, device, dim=dim)
-    sv = _heads(op, "v", v, q.dtype, device, k.shape[0], k.shape[1], dim)
-    _index(op, "cu_q", cu_q, None, device)
-    _index(op, "cu_k", cu_k, cu_q.shape[0], device)
-    if cu_q.shape[0] < 1:
+    k_token, k_head = _heads(op, "k", k, dtype, device, None, None, dim)
+    keys, kv_heads, _ = k.shape
+    v_token, v_head = _heads(op, "v", v, dtype, device, keys, kv_heads, dim)
+    offsets = _index(op, "cu_q", cu_q, None, device)
+    _index(op, "cu_k", cu_k, offsets, device)
+    if offsets < 1:
         _refuse(L.TB_ERR_SHAPE_MISMATCH, f"{op}: cu_q needs batch + 1 offsets")
     if out is None:
-        out, so = torch.empty((rows, heads, dim), dtype=q.dtype, device=device), (heads * dim, dim)
+        out, o_token, o_head = torch.empty((rows, heads, dim), dtype=dtype, device=q.device), heads * dim, dim
     else:
-        so = _heads(op, "out", out, q.dtype, device, rows, heads, dim)
+        o_token, o_head = _heads(op, "out", out, dtype, device, rows, heads, dim)
     if lse is None:
-        lse = torch.empty((heads, rows), dtype=torch.float32, device=device)
-    elif lse.dtype != torch.float32 or tuple(lse.shape) != (heads, rows) or not lse.is_contiguous() or lse.device != device:
-        _refuse(L.TB_ERR_SHAPE_MISMATCH, f"{op}: lse must be contiguous float32 of ({heads}, {rows})")
-    d = L.AttentionDesc(code, cu_q.shape[0] - 1, heads, k.shape[1], dim, int(bool(causal)),
-                        1.0 / math.sqrt(dim) if scale is None else scale, rows, k.shape[0],
-                        sq, sk, sv, so)
-    s = _on(stream, (q, k, v, cu_q, cu_k, out, lse))
-    L.check(L.load().tb_attention(ctx.h, ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(),
-                                  cu_k.data_ptr(), out.data_ptr(), lse.data_ptr(), s))
+        lse = torch.empty((heads, rows), dtype=_F32, device=q.device)
+    else:
+        _sums(op, lse, heads, rows, device)
+    d = L.AttentionDesc(code, offsets - 1, heads, kv_heads, dim, 1 if causal else 0, dim ** -0.5 if scale is None else scale,
+                        rows, keys, q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head)
+    L.check(L.load().tb_attention(ctx.h, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+                          out.data_ptr(), lse.data_ptr(), _on(stream, device, q, k, v, cu_q, cu_k, out, lse)))
     return out, lse
 
 
@@ -132,7 +154,8 @@ class PagedCache:
         self.ctx = ctx
         self.k_pages, self.v_pages = k_pages, v_pages
         self.page_table, self.lengths, self.refs = page_table, lengths, refs
-        self._default_scale = 1.0 / math.sqrt(head_dim)
+        self._device = k_pages.get_device()
+        self._lib = L.load()
         d = L.CacheDesc(code, layers, kv_heads, head_dim, page_size, num_pages, page_table.shape[0], page_table.shape[1])
         b = L.CacheBuffers(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), refs.data_ptr())
         h = ctypes.c_void_p()
@@ -162,67 +185,74 @@ class PagedCache:
             pass
 
     def _slots(self, op, name, t, n=None):
-        _index(op, name, t, n, self.k_pages.device)
-        return t.data_ptr()
+        return _index(op, name, t, n, self._device)
 
     def reserve(self, slots, counts=None, *, stream=None):
         """Grow slots[i] by counts[i] tokens (one each by default)."""
-        p = self._slots("cache reserve", "slots", slots)
-        c = None if counts is None else self._slots("cache reserve", "counts", counts, slots.shape[0])
-        L.check(L.load().tb_cache_reserve(self.h, p, c, slots.shape[0], _on(stream, (slots, counts))))
+        n = self._slots("cache reserve", "slots", slots)
+        if counts is not None:
+            self._slots("cache reserve", "counts", counts, n)
+        L.check(self._lib.tb_cache_reserve(self.h, slots.data_ptr(), None if counts is None else counts.data_ptr(), n,
+                                           _on(stream, self._device, slots, counts)))
 
     def write(self, layer, slots, offsets, k, v, *, stream=None):
         """Rows offsets[i]..offsets[i+1] of k and v are the last tokens of slots[i]."""
-        op = "cache write"
-        p = self._slots(op, "slots", slots)
-        o = self._slots(op, "offsets", offsets, slots.shape[0] + 1)
-        pages = self.k_pages
-        sk = _heads(op, "k", k, pages.dtype, pages.device, None, pages.shape[2], pages.shape[4])
-        sv = _heads(op, "v", v, pages.dtype, pages.device, k.shape[0], pages.shape[2], pages.shape[4])
-        L.check(L.load().tb_cache_write(self.h, layer, p, o, slots.shape[0], k.shape[0], k.data_ptr(), *sk, v.data_ptr(), *sv,
-                                        _on(stream, (slots, offsets, k, v))))
+        op, device = "cache write", self._device
+        n = self._slots(op, "slots", slots)
+        self._slots(op, "offsets", offsets, n + 1)
+        _, _, heads, _, dim = self.k_pages.shape
+        dtype = self.k_pages.dtype
+        k_token, k_head = _heads(op, "k", k, dtype, device, None, heads, dim)
+        rows = k.shape[0]
+        v_token, v_head = _heads(op, "v", v, dtype, device, rows, heads, dim)
+        L.check(self._lib.tb_cache_write(self.h, layer, slots.data_ptr(), offsets.data_ptr(), n, rows, k.data_ptr(),
+                                         k_token, k_head, v.data_ptr(), v_token, v_head,
+                                         _on(stream, device, slots, offsets, k, v)))
 
     def attend(self, layer, slots, q, *, scale=None, out=None, lse=None, stream=None):
         """Attention of one new token q [n, q_heads, head_dim] a slot. Returns (out, lse), out like q,
         lse float32 [n, q_heads]."""
-        op = "cache attend"
-        p = self._slots(op, "slots", slots)
-        pages = self.k_pages
-        n, heads, dim = slots.shape[0], q.shape[1] if q.dim() == 3 else 0, pages.shape[4]
-        sq = _heads(op, "q", q, pages.dtype, pages.device, n, None, dim)
+        op, device = "cache attend", self._device
+        n = self._slots(op, "slots", slots)
+        dtype, dim = self.k_pages.dtype, self.k_pages.shape[4]
+        q_seq, q_head = _heads(op, "q", q, dtype, device, n, None, dim)
+        heads = q.shape[1]
         if out is None:
-            out, so = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device), (heads * dim, dim)
+            out, o_seq, o_head = torch.empty((n, heads, dim), dtype=dtype, device=q.device), heads * dim, dim
         else:
-            so = _heads(op, "out", out, q.dtype, q.device, n, heads, dim)
+            o_seq, o_head = _heads(op, "out", out, dtype, device, n, heads, dim)
         if lse is None:
-            lse = torch.empty((n, heads), dtype=torch.float32, device=q.device)
-        elif lse.dtype != torch.float32 or tuple(lse.shape) != (n, heads) or not lse.is_contiguous() or lse.device != q.device:
-            _refuse(L.TB_ERR_SHAPE_MISMATCH, f"{op}: lse must be contiguous float32 of ({n}, {heads})")
-        L.check(L.load().tb_cache_attend(self.h, layer, p, n, heads, self._default_scale if scale is None else scale,
-                                         q.data_ptr(), *sq, out.data_ptr(), *so, lse.data_ptr(), _on(stream, (slots, q, out, lse))))
+            lse = torch.empty((n, heads), dtype=_F32, device=q.device)
+        else:
+            _sums(op, lse, n, heads, device)
+        L.check(self._lib.tb_cache_attend(self.h, layer, slots.data_ptr(), n, heads, dim ** -0.5 if scale is None else scale,
+                                          q.data_ptr(), q_seq, q_head, out.data_ptr(), o_seq, o_head, lse.data_ptr(),
+                                          _on(stream, device, slots, q, out, lse)))
         return out, lse
 
     def fork(self, parents, children, *, stream=None):
         """children[i] becomes a copy of parents[i]; full pages are shared."""
-        p = self._slots("cache fork", "parents", parents)
-        c = self._slots("cache fork", "children", children, parents.shape[0])
-        L.check(L.load().tb_cache_fork(self.h, p, c, parents.shape[0], _on(stream, (parents, children))))
+        n = self._slots("cache fork", "parents", parents)
+        self._slots("cache fork", "children", children, n)
+        L.check(self._lib.tb_cache_fork(self.h, parents.data_ptr(), children.data_ptr(), n,
+                                        _on(stream, self._device, parents, children)))
 
     def free(self, slots, *, stream=None):
         """Empty the slots."""
-        p = self._slots("cache free", "slots", slots)
-        L.check(L.load().tb_cache_free(self.h, p, slots.shape[0], _on(stream, (slots,))))
+        n = self._slots("cache free", "slots", slots)
+        L.check(self._lib.tb_cache_free(self.h, slots.data_ptr(), n, _on(stream, self._device, slots)))
 
     def copy_pages(self, src, dst, *, stream=None):
         """Copy the contents of pages src[i] to pages dst[i]."""
-        p = self._slots("cache copy_pages", "src", src)
-        o = self._slots("cache copy_pages", "dst", dst, src.shape[0])
-        L.check(L.load().tb_cache_copy_pages(self.h, p, o, src.shape[0], _on(stream, (src, dst))))
+        n = self._slots("cache copy_pages", "src", src)
+        self._slots("cache copy_pages", "dst", dst, n)
+        L.check(self._lib.tb_cache_copy_pages(self.h, src.data_ptr(), dst.data_ptr(), n, _on(stream, self._device, src, dst)))
 
     def compact(self, page_table=None, refs=None, *, stream=None):
         """Move the pages in use to the front, in place or with the new table and counts in other tensors."""
         for name, t, own in (("page_table", page_table, self.page_table), ("refs", refs, self.refs)):
-            if t is not None and (t.dtype != torch.int32 or t.shape != own.shape or not t.is_contiguous() or t.device != own.device):
+            if t is not None and (t.dtype is not _INT32 or t.shape != own.shape or not t.is_contiguous() or t.get_device() != self._device):
                 _refuse(L.TB_ERR_SHAPE_MISMATCH, f"cache compact: {name} must be like the cache's own")
-        L.check(L.load().tb_cache_compact(self.h, None if page_table is None else page_table.data_ptr(),
-                                          None if refs is None else refs.data_ptr(), _on(stream, (page_table, refs))))
+        L.check(self._lib.tb_cache_compact(self.h, None if page_table is None else page_table.data_ptr(),
+                                           None if refs is None else refs.data_ptr(),
+                                           _on(stream, self._device, page_table, refs)))

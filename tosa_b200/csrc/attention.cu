@@ -8,20 +8,24 @@
 // most 2^8, far inside the range of both types, and since weights and their sum share m the result
 // does not depend on it. lse = (m + log2 l) ln 2.
 //
-// A CTA takes two tiles of 128 rows (two heads of one key head's group, or two row tiles of one
-// head) that walk the same blocks of 128 keys. 12 warps:
+// An item is two tiles of 128 rows (two heads of one key head's group, or two row tiles of one head) that
+// walk the same blocks of 128 keys. One CTA an SM takes item after item: the grid has a block for each,
+// and a running CTA takes over blocks that have not begun, heaviest first within a sequence. 12 warps:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one row a thread: read the scores from tensor memory, write
 //                   the weights back to it as f16 / bf16, rescale o there when m moves, and store the
-//                   result at the end
+//                   result at the item's end
 //   warp 8          issues the MMAs: S = Q K^T (both from shared memory), O += P V (P from tensor memory)
-//   warp 9          TMA loads: the Q tiles, then K and V blocks through a ring
+//   warp 9          finds the items and loads by TMA: the Q tiles, then K and V blocks through a ring,
+//                   running ahead into the next item
 //   warps 10-11     look through the V blocks that some row sees only in part (see guard_block)
 // While one tile's softmax runs, the tensor cores work on the other tile. Tensor memory: S of both
 // tiles (128 columns each; P takes the first 64 of its S once the scores have been read) and O.
 //
 // Per tile and block the MMAs take 2 * 128 * 128 * head_dim multiply-adds (1024 cycles at head_dim 128)
-// and the 128 * 128 exponentials 1024 cycles of the special-function units, so the two are level and
-// neither may wait for the other.
+// and the 128 * 128 exponentials 1024 cycles of the special-function units. A tile's chain is softmax,
+// then O += P V, then the next S, so what counts is the softmax's length beside the other tile's MMAs:
+// part of the exponentials is computed as a polynomial on the otherwise idle FMA units, and the
+// first half of the weights is handed over while the second half is computed.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -44,6 +48,10 @@ static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "
 constexpr float kGrowth = 8.f;  // m follows the maximum when it has grown by more than this (powers of two)
 constexpr long long kDrainCycles = 2000000000ll;  // bound on a CTA's waits for its own copies and MMAs at its end
 constexpr int kGuards = 4;
+constexpr int kItems = 2;       // items announced at a time
+constexpr int kItemReaders = 11;  // warps that read an item: softmax, MMA, guards
+// Of every 8 pairs of exponentials this many are polynomials (see the kernel's head).
+constexpr int kPolyPairs = 3;
 
 // DCH: 64-element chunks of head_dim.
 template <int DCH>
@@ -51,18 +59,28 @@ struct PromptCfg {
     static constexpr int kChunk = kRows * 128;        // one chunk of a tile: 128 rows of 128 bytes, swizzled
     static constexpr int kTile = DCH * kChunk;
     static constexpr int kStages = DCH == 2 ? 5 : 8;  // ring of K and V blocks
-    static constexpr int kSmem = 1024 + (2 + kStages) * kTile;
+    static constexpr int kTiles = (2 + kStages) * kTile;
+};
+
+// A guarded value that is not finite is noted by its key, counted from the item's first guarded block.
+constexpr uint32_t kNoKey = 0xFFFFu;
+
+struct Item {
+    int valid, q0, k0, lq, lk, sub, kv_head;  // sub: the first tile's number among (row tile, head of the group)
 };
 
 struct PromptShared {
-    uint64_t q_full[2], full[8], empty[8], guard[kGuards], guard_done, s_full[2], p_full[2], o_full[2], drain;
+    alignas(16) uint4 response;  // of cancel_next_block
+    uint64_t q_full[2], q_empty[2], full[8], empty[8], guard[kGuards], s_full[2], p_half[2], p_full[2], o_full[2], drain;
+    uint64_t item_full[kItems], item_empty[kItems], guard_done[kItems], next;
     uint32_t tmem;
     int abort;
-    int seq, item;           // this CTA's sequence and item in it; seq < 0: none
-    int scan[13];
-    int odd;                 // some guarded value is not finite
-    int first[3][kKeys];     // per dimension: the first guarded key with NaN, +inf, -inf
+    Item item[kItems];
+    int odd[kItems];                          // some guarded value of the item is not finite
+    uint32_t first[kItems][3][kKeys / 2];     // per dimension (16 bits): the first key with NaN, +inf, -inf
 };
+static_assert(sizeof(PromptShared) + PromptCfg<2>::kTiles <= 232448 && sizeof(PromptShared) + PromptCfg<1>::kTiles <= 232448,
+              "shared memory above 227 KB");
 
 struct PromptArgs {
     void* out;
@@ -83,37 +101,40 @@ struct Tile {
     int seen_by_all;  // keys that every row sees (the first row's)
 };
 
-__device__ __forceinline__ int visible(const PromptArgs& a, int row, int lq, int lk) {
-    if (!a.causal) return lk;
-    return max(0, min(lk, row + lk - lq + 1));
+__device__ __forceinline__ int visible(int causal, int row, int lq, int lk) {
+    return causal ? max(0, min(lk, row + lk - lq + 1)) : lk;
 }
 
-__device__ __forceinline__ Tile tile_of(const PromptArgs& a, int sub, int kv_head, int lq, int lk) {
-    Tile t{0, 0, 0, 0, 0};
-    const int rt = sub / a.group;
-    t.row0 = rt * kRows;
-    t.rows = min(kRows, lq - t.row0);
-    if (t.rows <= 0) {
-        t.rows = 0;
-        t.seen_by_all = INT32_MAX;
-        return t;
+__device__ __forceinline__ Tile tile_of(const PromptArgs& a, const Item& it, int t) {
+    Tile x{0, 0, 0, 0, INT32_MAX};
+    const int sub = it.sub + t, rt = sub / a.group;
+    x.row0 = rt * kRows;
+    x.rows = min(kRows, it.lq - x.row0);
+    if (x.rows <= 0) {
+        x.rows = 0;
+        return x;
     }
-    t.head = kv_head * a.group + (sub - rt * a.group);
-    t.blocks = (visible(a, t.row0 + t.rows - 1, lq, lk) + kKeys - 1) / kKeys;
-    t.seen_by_all = visible(a, t.row0, lq, lk);
-    return t;
+    x.head = it.kv_head * a.group + (sub - rt * a.group);
+    x.blocks = (visible(a.causal, x.row0 + x.rows - 1, it.lq, it.lk) + kKeys - 1) / kKeys;
+    x.seen_by_all = visible(a.causal, x.row0, it.lq, it.lk);
+    return x;
+}
+
+// The first block of keys that some row of a tile that takes it does not see whole.
+__device__ __forceinline__ int first_guarded(const Tile& x, const Tile& y) {
+    return min(x.blocks > 0 ? x.seen_by_all / kKeys : INT32_MAX, y.blocks > 0 ? y.seen_by_all / kKeys : INT32_MAX);
 }
 
 // A weight of 0 does not take a key out of a product when the value is NaN or infinite. In a block
 // that some row sees only in part, V is therefore put in order before the MMA reads it: rows past the
 // sequence's end become zero, and values that are not finite become zero with their place noted
-// (first[]), to be added by the rows that do see them when they store their result. 64 threads.
+// (first[]), to be added by the rows that do see them when they store their result. 64 threads, a few
+// hundred cycles that the ring's depth hides. `rel`: the block's first key counted from first_guarded.
 template <bool BF16, int DCH>
-__device__ void guard_block(PromptShared& sh, uint8_t* v, int first_key, int lk, int head_dim, int t) {
+__device__ void guard_block(PromptShared& sh, int slot, uint8_t* v, int live, int rel, int t) {
     constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u;   // exponent of both halves
     constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u;   // all ones + 1: a carry into bit 15
     constexpr uint32_t kFrac = BF16 ? 0x7Fu : 0x3FFu;
-    const int live = lk - first_key;  // rows of the block inside the sequence
 #pragma unroll 4
     for (int i = t; i < DCH * kKeys * 8; i += 64) {
         const int row = (i >> 3) & (kKeys - 1);
@@ -132,21 +153,49 @@ __device__ void guard_block(PromptShared& sh, uint8_t* v, int first_key, int lk,
             const uint32_t h = (w[e >> 1] >> ((e & 1) * 16)) & 0xFFFFu;
             if ((h & (kExp & 0xFFFFu)) != (kExp & 0xFFFFu)) continue;
             const int kind = (h & kFrac) ? 0 : ((h >> 15) ? 2 : 1);
-            atomicMin(&sh.first[kind][d0 + e], first_key + row);
+            const uint32_t key = min(static_cast<uint32_t>(rel + row), kNoKey - 1), shift = (e & 1) * 16;
+            uint32_t* word = &sh.first[slot][kind][(d0 + e) >> 1];
+            uint32_t old = *word;
+            while (((old >> shift) & 0xFFFFu) > key) {  // ends: the half only gets smaller
+                const uint32_t seen = atomicCAS(word, old, (old & ~(0xFFFFu << shift)) | (key << shift));
+                if (seen == old) break;
+                old = seen;
+            }
             w[e >> 1] &= (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
-            sh.odd = 1;
+            sh.odd[slot] = 1;
         }
         *p = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
-__device__ __forceinline__ void tmem_ld_row(uint32_t taddr, uint32_t (&s)[128]) {
+struct RingPos {
+    int s = 0;
+    uint32_t ph = 0;
+    template <int S>
+    __device__ __forceinline__ void step() {
+        if (++s == S) {
+            s = 0;
+            ph ^= 1;
+        }
+    }
+};
+
+// Weights 2^(t - base) of 64 scores as 32 packed pairs, and their sum.
+template <bool BF16, int POLY>
+__device__ __forceinline__ void weights(const float* x, uint64_t scale, uint64_t neg_base, uint64_t (&sum)[2], uint32_t (&p)[32]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(taddr + 32 * c, r);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) s[32 * c + i] = r[i];
+    for (int i = 0; i < 32; ++i) {
+        const uint64_t t = fma_pair(pair_of(x[2 * i], x[2 * i + 1]), scale, neg_base);
+        float u, w;
+        if ((i & 7) >= 8 - POLY) {
+            exp2_poly(t, u, w);
+        } else {
+            split_pair(t, u, w);
+            u = exp2_fast(u);
+            w = exp2_fast(w);
+        }
+        sum[i & 1] = add_pair(sum[i & 1], pair_of(u, w));
+        p[i] = pack2<BF16>(u, w);
     }
 }
 
@@ -156,18 +205,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const __grid_constant__ CUtensorMap tmV, const PromptArgs a) {
     using Cfg = PromptCfg<DCH>;
     constexpr int S = Cfg::kStages;
-    extern __shared__ uint8_t raw[];
-    __shared__ PromptShared sh;
-    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* sq = base;
-    uint8_t* ring = base + 2 * Cfg::kTile;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    extern __shared__ __align__(1024) uint8_t sq[];  // Q tiles, ring, PromptShared
+    uint8_t* ring = sq + 2 * Cfg::kTile;
+    PromptShared& sh = *reinterpret_cast<PromptShared*>(sq + Cfg::kTiles);
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     volatile int* abort_flag = &sh.abort;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], 1);
+            mbar_init(&sh.q_empty[i], 1);
             mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.p_half[i], 4);
             mbar_init(&sh.p_full[i], 4);
             mbar_init(&sh.o_full[i], 1);
         }
@@ -176,202 +225,334 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sh.empty[i], 1);
         }
         for (int i = 0; i < kGuards; ++i) mbar_init(&sh.guard[i], 2);
-        mbar_init(&sh.guard_done, 2);
+        for (int i = 0; i < kItems; ++i) {
+            mbar_init(&sh.item_full[i], 1);
+            mbar_init(&sh.item_empty[i], kItemReaders);
+            mbar_init(&sh.guard_done[i], 2);
+            sh.odd[i] = 1;  // first[] is cleared before the first use
+        }
+        mbar_init(&sh.next, 1);
         mbar_init(&sh.drain, 1);
         fence_mbar_init();
         sh.abort = 0;
-        sh.seq = -1;
-        sh.odd = 0;
     }
-    for (int i = threadIdx.x; i < 3 * kKeys; i += kThreads) (&sh.first[0][0])[i] = INT32_MAX;
     if (warp == 8) {
         tmem_alloc(&sh.tmem, 512);
         tmem_relinquish();
-        if (lane == 0) {
-            tma_prefetch_desc(&tmQ);
-            tma_prefetch_desc(&tmK);
-            tma_prefetch_desc(&tmV);
-        }
-    }
-    grid_dependency_wait();
-    // This CTA's item: items lie sequence behind sequence, ceil(row tiles * group / 2) for each.
-    const int kv_head = blockIdx.x % a.kv_heads;
-    const long long want = blockIdx.x / a.kv_heads;
-    {
-        long long before = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
-            const int b = b0 + threadIdx.x;
-            int items = 0;
-            if (b < a.batch) {
-                const long long q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
-                if (q0 < 0 || q1 < q0 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k) {
-                    if (blockIdx.x == 0) atomicOr(a.err, DEV_ERR_INDEX);
-                } else {
-                    items = static_cast<int>(((q1 - q0 + kRows - 1) / kRows * a.group + 1) >> 1);
-                }
-            }
-            int x = items;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            __syncthreads();
-            if (lane == 31) sh.scan[warp] = x;
-            __syncthreads();
-            int pre = 0, total = 0;
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) pre += sh.scan[w];
-                total += sh.scan[w];
-            }
-            const long long hi = before + pre + x, lo = hi - items;
-            if (lo <= want && want < hi) {
-                sh.seq = b;
-                sh.item = static_cast<int>(hi - 1 - want);  // the last rows, which see the most keys, first
-            }
-            before += total;
-            if (before > want) break;
-        }
+    } else if (warp == 9 && lane == 0) {
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    const int seq = sh.seq;
     const long long limit = a.timeout_cycles;
     const long long drain_limit = limit > kDrainCycles ? limit : kDrainCycles;
+    // A wait by a whole warp; its lanes agree on whether it gave up.
+    auto wait = [&](uint64_t* bar, uint32_t ph) {
+        return __all_sync(0xffffffffu, mbar_wait_bounded(bar, ph, abort_flag, limit)) != 0;
+    };
+    auto gave_up = [&]() {
+        if (lane == 0) {
+            atomicOr(a.err, DEV_ERR_TIMEOUT);
+            *abort_flag = 1;
+        }
+    };
+    // The k-th item, false at the end or when a wait gave up.
+    auto read_item = [&](int k, Item& it, bool& ok) {
+        ok = wait(&sh.item_full[k % kItems], (k / kItems) & 1);
+        if (!ok) return false;
+        it = sh.item[k % kItems];
+        return it.valid != 0;
+    };
+    auto done_with_item = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.item_empty[k % kItems]);
+    };
 
-    if (seq >= 0) {
-        const int q0 = a.cu_q[seq], k0 = a.cu_k[seq];
-        const int lq = a.cu_q[seq + 1] - q0, lk = a.cu_k[seq + 1] - k0;
-        const Tile tile[2] = {tile_of(a, 2 * sh.item, kv_head, lq, lk), tile_of(a, 2 * sh.item + 1, kv_head, lq, lk)};
-        const int blocks = max(tile[0].blocks, tile[1].blocks);
-
-        if (warp >= 8) {
-            setmaxnreg_dec<kOtherRegs>();
-            if (warp == 9 && lane == 0 && blocks > 0) {
-                // ------------------------------------------------------------ loads
-                for (int t = 0; t < 2; ++t) {
-                    if (tile[t].blocks == 0) continue;
-                    mbar_arrive_expect_tx(&sh.q_full[t], Cfg::kTile);
-                    for (int c = 0; c < DCH; ++c)
-                        tma_load_3d(sq + t * Cfg::kTile + c * Cfg::kChunk, &tmQ, &sh.q_full[t], 64 * c, tile[t].head,
-                                    q0 + tile[t].row0);
+    if (warp >= 8) {
+        setmaxnreg_dec<kOtherRegs>();
+        if (warp == 9) {
+            // ---------------------------------------------------------------- items and loads
+            grid_dependency_wait();
+            RingPos r;
+            uint32_t loads = 0, qn[2] = {0, 0};
+            bool ok = true;
+            int b0 = 0;            // sequences before b0 have `before` items (items come in rising order, as a rule)
+            long long before = 0;
+            int block = blockIdx.x;
+            for (int k = 0;; ++k) {
+                // items lie sequence behind sequence, ceil(row tiles * group / 2) for each
+                Item it{};
+                const long long want = block < 0 ? 0 : block / a.kv_heads;
+                if (want < before) before = b0 = 0;
+                while (block >= 0 && b0 < a.batch) {
+                    const int b = b0 + lane;
+                    int items = 0;
+                    long long q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+                    if (b < a.batch) {
+                        q0 = a.cu_q[b];
+                        q1 = a.cu_q[b + 1];
+                        k0 = a.cu_k[b];
+                        k1 = a.cu_k[b + 1];
+                        // (sequences out of range are reported by the first block's warp 10)
+                        if (!(q0 < 0 || q1 < q0 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k))
+                            items = static_cast<int>(((q1 - q0 + kRows - 1) / kRows * a.group + 1) >> 1);
+                    }
+                    int x = items;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int y = __shfl_up_sync(0xffffffffu, x, o);
+                        if (lane >= o) x += y;
+                    }
+                    const unsigned over = __ballot_sync(0xffffffffu, before + x > want);
+                    if (over) {
+                        const int l = __ffs(over) - 1;
+                        it.valid = 1;
+                        it.q0 = __shfl_sync(0xffffffffu, static_cast<int>(q0), l);
+                        it.k0 = __shfl_sync(0xffffffffu, static_cast<int>(k0), l);
+                        it.lq = __shfl_sync(0xffffffffu, static_cast<int>(q1), l) - it.q0;
+                        it.lk = __shfl_sync(0xffffffffu, static_cast<int>(k1), l) - it.k0;
+                        // the last rows, which see the most keys, first
+                        it.sub = 2 * static_cast<int>(before + __shfl_sync(0xffffffffu, x, l) - 1 - want);
+                        it.kv_head = block - static_cast<int>(want) * a.kv_heads;
+                        break;
+                    }
+                    before += __shfl_sync(0xffffffffu, x, 31);
+                    b0 += 32;
                 }
-                int it = 0, s = 0;
-                uint32_t ph = 0;
-                bool ok = true;
-                for (; it < 2 * blocks; ++it) {
-                    if (!mbar_wait_bounded(&sh.empty[s], ph ^ 1, abort_flag, limit)) { ok = false; break; }
-                    mbar_arrive_expect_tx(&sh.full[s], Cfg::kTile);
-                    const CUtensorMap* m = (it & 1) ? &tmV : &tmK;
-                    for (int c = 0; c < DCH; ++c)
-                        tma_load_3d(ring + s * Cfg::kTile + c * Cfg::kChunk, m, &sh.full[s], 64 * c, kv_head,
-                                    k0 + (it >> 1) * kKeys);
-                    if (++s == S) { s = 0; ph ^= 1; }
+                const int slot = k % kItems;
+                ok = wait(&sh.item_empty[slot], ((k / kItems) & 1) ^ 1);
+                if (!ok) break;
+                if (sh.odd[slot]) {  // the slot's last item noted keys: cleared now that its readers are done
+                    for (int i = lane; i < 3 * kKeys / 2; i += 32) (&sh.first[slot][0][0])[i] = 0xFFFFFFFFu;
+                    __syncwarp();
+                    if (lane == 0) sh.odd[slot] = 0;
                 }
-                if (!ok) { atomicOr(a.err, DEV_ERR_TIMEOUT); *abort_flag = 1; }
-                // every issued load lands before the CTA may exit
-                for (int t = 0; t < 2; ++t)
-                    if (tile[t].blocks) mbar_wait_bounded(&sh.q_full[t], 0, nullptr, drain_limit);
-                for (int i = it > S ? it - S : 0; i < it; ++i)
-                    mbar_wait_bounded(&sh.full[i % S], (i / S) & 1, nullptr, drain_limit);
-            } else if (warp == 8 && lane == 0 && blocks > 0) {
-                // ------------------------------------------------------------ MMAs
-                const uint32_t idesc_s = idesc_f16(kRows, kKeys, BF16, false);
-                const uint32_t idesc_o = idesc_f16(kRows, a.head_dim, BF16, true);
-                const int ksteps = a.head_dim / 16;
-                bool ok = true;
-                auto wait = [&](uint64_t* bar, uint32_t ph) {
-                    if (ok && !mbar_wait_bounded(bar, ph, abort_flag, limit)) ok = false;
-                    return ok;
+                if (lane == 0) sh.item[slot] = it;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.item_full[slot]);
+                if (!it.valid) break;
+                if (lane == 0) {  // the next item's block, while this one loads
+                    fence_proxy_async_smem();
+                    mbar_arrive_expect_tx(&sh.next, 16);
+                    cancel_next_block(&sh.response, &sh.next);
+                }
+                const Tile tile[2] = {tile_of(a, it, 0), tile_of(a, it, 1)};
+                const int blocks = max(tile[0].blocks, tile[1].blocks);
+                auto load_block = [&](const CUtensorMap* m, int j) {
+                    ok = wait(&sh.empty[r.s], r.ph ^ 1);
+                    if (!ok) return;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.full[r.s], Cfg::kTile);
+#pragma unroll
+                        for (int c = 0; c < DCH; ++c)
+                            tma_load_3d(ring + r.s * Cfg::kTile + c * Cfg::kChunk, m, &sh.full[r.s], 64 * c, it.kv_head, it.k0 + j * kKeys);
+                    }
+                    __syncwarp();
+                    ++loads;
+                    r.step<S>();
                 };
-                auto scores = [&](int t, int stage) {
-                    const uint32_t qa = smem_u32(sq + t * Cfg::kTile), kb = smem_u32(ring + stage * Cfg::kTile);
-                    for (int k = 0; k < ksteps; ++k) {
-                        const uint32_t o = (k >> 2) * Cfg::kChunk + (k & 3) * 32;
-                        tc_mma<1>(tmem + t * 128, smem_desc(qa + o, 16, 1024, 2), smem_desc(kb + o, 16, 1024, 2), idesc_s, k > 0);
+                for (int t = 0; t < 2 && ok; ++t) {
+                    if (tile[t].blocks == 0) continue;
+                    ok = wait(&sh.q_empty[t], (qn[t] & 1) ^ 1);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.q_full[t], Cfg::kTile);
+#pragma unroll
+                        for (int c = 0; c < DCH; ++c)
+                            tma_load_3d(sq + t * Cfg::kTile + c * Cfg::kChunk, &tmQ, &sh.q_full[t], 64 * c, tile[t].head, it.q0 + tile[t].row0);
+                    }
+                    __syncwarp();
+                    ++qn[t];
+                    if (t == 0) load_block(&tmK, 0);
+                }
+                if (ok && tile[0].blocks == 0 && blocks > 0) load_block(&tmK, 0);
+                for (int j = 0; j < blocks && ok; ++j) {
+                    load_block(&tmV, j);
+                    if (ok && j + 1 < blocks) load_block(&tmK, j + 1);
+                }
+                // the answer is read even when a wait gave up: it must not arrive after the CTA's end
+                const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.next, k & 1, nullptr, drain_limit));
+                if (!ok || !got) {
+                    ok = false;
+                    break;
+                }
+                block = cancelled_block(&sh.response);
+                __syncwarp();
+            }
+            if (!ok) gave_up();
+            // every issued load lands before the CTA may exit
+            for (int t = 0; t < 2; ++t)
+                if (qn[t]) mbar_wait_bounded(&sh.q_full[t], (qn[t] - 1) & 1, nullptr, drain_limit);
+            for (uint32_t i = loads > S ? loads - S : 0; i < loads; ++i)
+                mbar_wait_bounded(&sh.full[i % S], (i / S) & 1, nullptr, drain_limit);
+        } else if (warp == 8) {
+            // ---------------------------------------------------------------- MMAs
+            // The whole warp walks along and one lane issues: descriptors then stay in uniform
+            // registers, and a run of MMAs is issued faster than the tensor cores take them.
+            const uint32_t idesc_s = idesc_f16(kRows, kKeys, BF16, false);
+            const uint32_t idesc_o = idesc_f16(kRows, a.head_dim, BF16, true);
+            const uint64_t dq = smem_desc(smem_u32(sq), 16, 1024, 2);             // K-major: Q, K
+            const uint64_t dk = smem_desc(smem_u32(ring), 16, 1024, 2);
+            const uint64_t dv = smem_desc(smem_u32(ring), Cfg::kChunk, 1024, 2);  // dimension-major: V
+            const int ksteps = a.head_dim / 16;
+            const bool leader = elect_one();
+            auto scores = [&](int t, int stage) {
+                const uint64_t qa = dq + ((t * Cfg::kTile) >> 4), kb = dk + ((stage * Cfg::kTile) >> 4);
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < 4 * DCH; ++k) {
+                        const uint32_t o = ((k >> 2) * Cfg::kChunk + (k & 3) * 32) >> 4;
+                        if (k < ksteps) tc_mma<1>(tmem + t * 128, qa + o, kb + o, idesc_s, k > 0);
                     }
                     tc_commit(&sh.s_full[t]);
-                };
-                auto product = [&](int t, int stage, bool first) {
-                    const uint32_t vb = smem_u32(ring + stage * Cfg::kTile);
-#pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8,
-                                      smem_desc(vb + k * 2048, Cfg::kChunk, 1024, 2), idesc_o, !first || k > 0);
-                };
-                wait(&sh.full[0], 0);
-                for (int t = 0; t < 2; ++t)
-                    if (tile[t].blocks && wait(&sh.q_full[t], 0)) {
-                        tc_fence_after();
-                        scores(t, 0);
-                    }
-                tc_commit(&sh.empty[0]);
-                int it = 1;  // V block j is ring entry 2 j + 1, the next K block 2 j + 2
-                for (int j = 0; j < blocks && ok; ++j, it += 2) {
-                    const int sv = it % S, sk = (it + 1) % S;
-                    const uint32_t pv = (it / S) & 1, pk = ((it + 1) / S) & 1;
-                    wait(&sh.full[sv], pv);
-                    wait(&sh.guard[j % kGuards], (j / kGuards) & 1);
-                    for (int t = 0; t < 2 && ok; ++t) {
-                        if (j < tile[t].blocks && wait(&sh.p_full[t], j & 1)) {
-                            tc_fence_after();
-                            product(t, sv, j == 0);
-                            if (j + 1 == tile[t].blocks) tc_commit(&sh.o_full[t]);
-                        }
-                        if (t == 1) tc_commit(&sh.empty[sv]);
-                        if (j + 1 < tile[t].blocks && wait(&sh.full[sk], pk)) {
-                            tc_fence_after();
-                            scores(t, sk);
-                        }
-                    }
-                    if (j + 1 < blocks) tc_commit(&sh.empty[sk]);
                 }
-                if (!ok) { atomicOr(a.err, DEV_ERR_TIMEOUT); *abort_flag = 1; }
-                tc_commit(&sh.drain);
-                mbar_wait_bounded(&sh.drain, 0, nullptr, drain_limit);
-            } else if (warp >= 10) {
-                // ------------------------------------------------------------ V blocks seen in part
-                bool ok = true;
-                for (int j = 0; j < blocks && ok; ++j) {
-                    const int it = 2 * j + 1;
+                __syncwarp();
+            };
+            auto product = [&](int t, int stage, int half, bool first) {
+                const uint64_t vb = dv + ((stage * Cfg::kTile) >> 4);
+                if (leader) {
+#pragma unroll
+                    for (int i = 0; i < kKeys / 32; ++i) {
+                        const int k = half * (kKeys / 32) + i;
+                        tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vb + ((k * 2048) >> 4), idesc_o, !first || k > 0);
+                    }
+                }
+                __syncwarp();
+            };
+            auto commit = [&](uint64_t* bar) {
+                if (leader) tc_commit(bar);
+                __syncwarp();
+            };
+            RingPos r;                     // the K block at hand, then its V block, ...
+            uint32_t n[2] = {0, 0};        // blocks of each tile so far
+            uint32_t qn[2] = {0, 0}, vn = 0;
+            bool ok = true;
+            Item it;
+            for (int k = 0; read_item(k, it, ok); ++k) {
+                done_with_item(k);
+                const Tile tile[2] = {tile_of(a, it, 0), tile_of(a, it, 1)};
+                const int blocks = max(tile[0].blocks, tile[1].blocks);
+                if (blocks == 0) continue;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (ok && tile[t].blocks) {
+                        ok = wait(&sh.q_full[t], qn[t]++ & 1) && wait(&sh.full[r.s], r.ph);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(t, r.s);
+                        if (tile[t].blocks == 1) commit(&sh.q_empty[t]);
+                    }
+                if (!ok) break;
+                commit(&sh.empty[r.s]);
+                r.step<S>();
+                for (int j = 0; j < blocks && ok; ++j, ++vn) {
+                    const RingPos v = r;
+                    r.step<S>();
+                    ok = wait(&sh.full[v.s], v.ph) && wait(&sh.guard[vn % kGuards], (vn / kGuards) & 1);
+                    if (!ok) break;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (j < tile[t].blocks) {
+                            ok = ok && wait(&sh.p_half[t], n[t] & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            //TR(40+t)
+                            product(t, v.s, 0, j == 0);
+                            ok = wait(&sh.p_full[t], n[t]++ & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            product(t, v.s, 1, false);
+                            //TR(42+t)
+                            if (j + 1 == tile[t].blocks) commit(&sh.o_full[t]);
+                        }
+                        if (t == 1) commit(&sh.empty[v.s]);
+                        if (j + 1 < tile[t].blocks) {
+                            ok = wait(&sh.full[r.s], r.ph);
+                            if (!ok) break;
+                            tc_fence_after();
+                            scores(t, r.s);
+                            //TR(44+t)
+                            if (j + 2 == tile[t].blocks) commit(&sh.q_empty[t]);
+                        }
+                    }
+                    if (!ok) break;
+                    if (j + 1 < blocks) {
+                        commit(&sh.empty[r.s]);
+                        r.step<S>();
+                    }
+                }
+                if (!ok) break;
+            }
+            if (!ok) gave_up();
+            commit(&sh.drain);
+            mbar_wait_bounded(&sh.drain, 0, nullptr, drain_limit);
+            __syncwarp();
+        } else {
+            // ---------------------------------------------------------------- V blocks seen in part
+            grid_dependency_wait();
+            if (blockIdx.x == 0 && warp == 10)
+                for (int b = lane; b < a.batch; b += 32) {
+                    const long long q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+                    if (q0 < 0 || q1 < q0 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k) atomicOr(a.err, DEV_ERR_INDEX);
+                }
+            RingPos r;
+            uint32_t vn = 0;
+            bool ok = true;
+            Item it;
+            for (int k = 0; read_item(k, it, ok); ++k) {
+                const Tile tile[2] = {tile_of(a, it, 0), tile_of(a, it, 1)};
+                const int blocks = max(tile[0].blocks, tile[1].blocks);
+                const int from = first_guarded(tile[0], tile[1]);
+                for (int j = 0; j < blocks; ++j, ++vn) {
+                    r.step<S>();  // past the K block
+                    ok = wait(&sh.full[r.s], r.ph);
+                    if (!ok) break;
                     // a tile that does not reach this block has no say in it
                     const int seen = min(j < tile[0].blocks ? tile[0].seen_by_all : INT32_MAX,
                                          j < tile[1].blocks ? tile[1].seen_by_all : INT32_MAX);
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.full[it % S], (it / S) & 1, abort_flag, limit));
-                    if (!ok) break;
                     if (seen < (j + 1) * kKeys) {
-                        guard_block<BF16, DCH>(sh, ring + (it % S) * Cfg::kTile, j * kKeys, lk, a.head_dim, threadIdx.x - 320);
+                        guard_block<BF16, DCH>(sh, k % kItems, ring + r.s * Cfg::kTile, it.lk - j * kKeys, (j - from) * kKeys, threadIdx.x - 320);
                         fence_proxy_async_smem();
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.guard[j % kGuards]);
+                    if (lane == 0) mbar_arrive(&sh.guard[vn % kGuards]);
+                    r.step<S>();
                 }
-                __syncwarp();
-                if (lane == 0) {
-                    if (!ok) { atomicOr(a.err, DEV_ERR_TIMEOUT); *abort_flag = 1; }
-                    mbar_arrive(&sh.guard_done);
-                }
-            }
-        } else {
-            // ------------------------------------------------------------ softmax
-            setmaxnreg_inc<kSoftmaxRegs>();
-            const int t = warp >> 2;
-            const Tile my = t ? tile[1] : tile[0];
-            const int r = threadIdx.x & 127;
-            const int row = my.row0 + r;
-            const int sees = r < my.rows ? visible(a, row, lq, lk) : lk;
-            const uint32_t ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * 128;
-            const uint32_t to = ts + 256;  // O
-            float m = -INFINITY, l = 0.f;
-            bool ok = true;
-            for (int j = 0; j < my.blocks; ++j) {
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.s_full[t], j & 1, abort_flag, limit));
                 if (!ok) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.guard_done[k % kItems]);
+                done_with_item(k);
+            }
+            if (!ok) gave_up();
+        }
+    } else {
+        // -------------------------------------------------------------------- softmax
+        setmaxnreg_inc<kSoftmaxRegs>();
+        grid_dependency_wait();
+        const int t = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * 128;
+        const uint32_t to = ts + 256;  // O
+        const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
+        uint32_t n = 0, outs = 0;  // blocks and results so far
+        bool ok = true;
+        Item it;
+        for (int k = 0; read_item(k, it, ok); ++k) {
+            const Tile my = tile_of(a, it, t);
+            const int row = my.row0 + r;
+            const int sees = r < my.rows ? visible(a.causal, row, it.lq, it.lk) : it.lk;
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < my.blocks; ++j, ++n) {
+                ok = wait(&sh.s_full[t], n & 1);
+                if (!ok) break;
+                //TR(warp)
                 tc_fence_after();
                 uint32_t s[128];
-                tmem_ld_row(ts, s);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
                 tmem_ld_wait();
                 float x[128];
 #pragma unroll
@@ -379,16 +560,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     asm volatile("" : "+r"(s[i]));
                     x[i] = __uint_as_float(s[i]);
                 }
-                if (my.seen_by_all < (j + 1) * kKeys) {
-                    const int n = sees - j * kKeys;
+                const bool part = my.seen_by_all < (j + 1) * kKeys;  // some row does not see the whole block
+                if (part) {
+                    const int seen = sees - j * kKeys;
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) x[i] = i < n ? x[i] : -INFINITY;
+                    for (int i = 0; i < 128; ++i) x[i] = i < seen ? x[i] : -INFINITY;
                 }
-                float top[4] = {x[0], x[1], x[2], x[3]};
+                //TR(8+warp)
+                float top[4];
 #pragma unroll
-                for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], x[i]);
-                const float m1 = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-                const bool grow = m1 > m + kGrowth;
+                for (int c = 0; c < 4; ++c) {
+                    top[c] = x[32 * c];
+#pragma unroll
+                    for (int i = 1; i < 31; i += 2) top[c] = max3_nan(top[c], x[32 * c + i], x[32 * c + i + 1]);
+                    top[c] = max_nan(top[c], x[32 * c + 31]);
+                }
+                // a NaN among the scores becomes the row's reference and with it the whole row
+                const float m1 = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * a.scale_log2;
+                const bool grow = !(m1 <= m + kGrowth);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float mm = grow ? m1 : m;
                     if (j > 0) {
@@ -409,73 +598,76 @@ __global__ void __launch_bounds__(kThreads, 1)
                     m = mm;
                 }
                 const float base = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                //TR(16+warp)
+                const uint64_t neg = pair_of(-base, -base);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t p[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float u = exp2_fast(fmaf(x[64 * c + 2 * i], a.scale_log2, -base));
-                        const float w = exp2_fast(fmaf(x[64 * c + 2 * i + 1], a.scale_log2, -base));
-                        sum[(2 * i) & 3] += u;
-                        sum[(2 * i + 1) & 3] += w;
-                        p[i] = pack2<BF16>(u, w);
-                    }
+                    // keys that are not seen get a weight of exactly 0 from the special-function unit
+                    if (part) weights<BF16, 0>(x + 64 * c, scale2, neg, sum, p);
+                    else weights<BF16, kPolyPairs>(x + 64 * c, scale2, neg, sum, p);
                     tmem_st_32x32b_x32(ts + 32 * c, p);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(c == 0 ? &sh.p_half[t] : &sh.p_full[t]);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[t]);
+                //TR(24+warp)
+                float s0, s1;
+                split_pair(add_pair(sum[0], sum[1]), s0, s1);
+                l += s0 + s1;
+                //TR(32+warp)
             }
-            if (my.blocks > 0 && ok)
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.o_full[t], 0, abort_flag, limit) &&
-                                                 mbar_wait_bounded(&sh.guard_done, 0, abort_flag, limit));
+            if (!ok) break;
+            ok = wait(&sh.guard_done[k % kItems], (k / kItems) & 1);
+            if (ok && my.blocks > 0) ok = wait(&sh.o_full[t], outs++ & 1);
+            if (!ok) break;
             tc_fence_after();
-            if (ok) {
-                const bool live = r < my.rows, any = sees > 0;
-                const float inv = any ? 1.f / l : 0.f;
-                const int odd = sh.odd;
-                uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(q0 + row) * a.o_token + my.head * a.o_head;
-                for (int c = 0; c < a.head_dim; c += 16) {
-                    uint32_t o[16];
-                    if (my.blocks > 0) {
-                        tmem_ld_32x32b_x16(to + c, o);
-                        tmem_ld_wait();
+            const bool live = r < my.rows, any = sees > 0;
+            // (a reference that is not finite: a score of NaN or +inf, or every score -inf)
+            const float inv = any ? (isfinite(m) ? 1.f / l : NAN) : 0.f;
+            const int odd = sh.odd[k % kItems];
+            const uint16_t* first = reinterpret_cast<const uint16_t*>(&sh.first[k % kItems][0][0]);
+            const int rel = odd ? sees - first_guarded(tile_of(a, it, 0), tile_of(a, it, 1)) * kKeys : 0;
+            uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(it.q0 + row) * a.o_token + my.head * a.o_head;
+            for (int c = 0; c < a.head_dim; c += 16) {
+                uint32_t o[16];
+                if (my.blocks > 0) {
+                    tmem_ld_32x32b_x16(to + c, o);
+                    tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(o[i]));
-                    } else {
+                    for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(o[i]));
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = 0;
-                    }
-                    if (odd) {
-                        for (int i = 0; i < 16; ++i) {
-                            float y = __uint_as_float(o[i]);
-                            if (sh.first[0][c + i] < sees) y = NAN;
-                            if (sh.first[1][c + i] < sees) y += INFINITY;
-                            if (sh.first[2][c + i] < sees) y -= INFINITY;
-                            o[i] = __float_as_uint(y);
-                        }
-                    }
-                    uint32_t h[8];
+                    for (int i = 0; i < 16; ++i) o[i] = 0;
+                }
+                if (odd) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        h[i] = any ? pack2<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
-                    if (live) {
-                        *reinterpret_cast<uint4*>(out + c) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+                    for (int i = 0; i < 16; ++i) {
+                        float y = __uint_as_float(o[i]);
+                        if (first[c + i] < rel) y = NAN;
+                        if (first[kKeys + c + i] < rel) y += INFINITY;
+                        if (first[2 * kKeys + c + i] < rel) y -= INFINITY;
+                        o[i] = __float_as_uint(y);
                     }
                 }
-                if (a.lse != nullptr && live)
-                    a.lse[static_cast<long long>(my.head) * a.total_q + q0 + row] =
-                        any ? ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2 : -INFINITY;
-            } else if (lane == 0) {
-                atomicOr(a.err, DEV_ERR_TIMEOUT);
-                *abort_flag = 1;
+                uint32_t h[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    h[i] = any ? pack2<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
+                if (live) {
+                    *reinterpret_cast<uint4*>(out + c) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+                }
             }
+            if (a.lse != nullptr && live)
+                a.lse[static_cast<long long>(my.head) * a.total_q + it.q0 + row] =
+                    any && m != -INFINITY ? (m + log2f(l)) * kLn2 : -INFINITY;
             tc_fence_before();
+            done_with_item(k);
         }
+        if (!ok) gave_up();
     }
     __syncthreads();
     if (warp == 8) {
@@ -498,9 +690,9 @@ tb_status attention_check(const char* op, int dtype, int q_heads, int kv_heads, 
 
 // [tokens][heads][head_dim] as {head_dim, heads, tokens}, boxes of 128 tokens by 64 elements of one head.
 static tb_status tile_map(CUtensorMap* m, const tb_attention_desc* d, const void* p, int64_t heads, int64_t tokens,
-                          const int64_t* stride) {
+                          int64_t token_stride, int64_t head_stride) {
     // the stride of a dimension of one element says nothing; the map wants a valid one
-    const uint64_t head = heads > 1 ? stride[1] : d->head_dim, token = tokens > 1 ? stride[0] : d->head_dim;
+    const uint64_t head = heads > 1 ? head_stride : d->head_dim, token = tokens > 1 ? token_stride : d->head_dim;
     const uint64_t dims[3] = {static_cast<uint64_t>(d->head_dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens)};
     const uint64_t strides[2] = {head * 2, token * 2};
     const uint32_t box[3] = {64, 1, kRows};
@@ -512,6 +704,7 @@ template <bool BF16, int DCH>
 static tb_status launch_prompt(tb_context* ctx, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                                const PromptArgs& a, long long grid, cudaStream_t st) {
     auto* kernel = prompt_kernel<BF16, DCH>;
+    constexpr int kSmem = PromptCfg<DCH>::kTiles + static_cast<int>(sizeof(PromptShared));
     static bool ready = false;  // the attribute is per function and process-wide
     if (!ready) {
         // the warpgroups re-split the registers of the launch (setmaxnreg), which needs all of them
@@ -519,13 +712,13 @@ static tb_status launch_prompt(tb_context* ctx, const CUtensorMap& q, const CUte
         TB_CUDA(cudaFuncGetAttributes(&fa, kernel));
         if (fa.numRegs < kLaunchRegs)
             return fail(TB_ERR_CUDA, "attention built with %d registers a thread; its register split needs %d", fa.numRegs, kLaunchRegs);
-        TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptCfg<DCH>::kSmem));
+        TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         ready = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = PromptCfg<DCH>::kSmem;
+    cfg.dynamicSmemBytes = kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -555,20 +748,21 @@ TB_API tb_status tb_attention(tb_context* ctx, const tb_attention_desc* d, const
     if (!q || !cu_q || !cu_k || !out || (d->total_k > 0 && (!k || !v)))
         return fail(TB_ERR_INVALID_ARGUMENT, "attention: null pointer");
     long long strides = 0;
-    for (const int64_t* s : {d->q_stride, d->k_stride, d->v_stride, d->out_stride}) {
-        if (s[0] < 0 || s[1] < 0) return fail(TB_ERR_SHAPE_MISMATCH, "attention: negative stride");
-        strides |= s[0] | s[1];
+    for (int64_t s : {d->q_token_stride, d->q_head_stride, d->k_token_stride, d->k_head_stride, d->v_token_stride,
+                      d->v_head_stride, d->out_token_stride, d->out_head_stride}) {
+        if (s < 0) return fail(TB_ERR_SHAPE_MISMATCH, "attention: negative stride");
+        strides |= s;
     }
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (strides & 7))
         return fail(TB_ERR_INVALID_ARGUMENT, "attention: tensors must be 16-byte aligned with strides that are multiples of 8");
     // without keys nothing is loaded; the maps are made of q's first row
     const bool keys = d->total_k > 0;
     CUtensorMap mq, mk, mv;
-    TB_TRY(tile_map(&mq, d, q, d->q_heads, d->total_q, d->q_stride));
-    TB_TRY(tile_map(&mk, d, keys ? k : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->k_stride));
-    TB_TRY(tile_map(&mv, d, keys ? v : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->v_stride));
+    TB_TRY(tile_map(&mq, d, q, d->q_heads, d->total_q, d->q_token_stride, d->q_head_stride));
+    TB_TRY(tile_map(&mk, d, keys ? k : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->k_token_stride, d->k_head_stride));
+    TB_TRY(tile_map(&mv, d, keys ? v : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->v_token_stride, d->v_head_stride));
     const int group = d->q_heads / d->kv_heads;
-    PromptArgs a{out, lse, cu_q, cu_k, d->out_stride[0], d->out_stride[1], d->total_q, d->total_k, d->batch, group,
+    PromptArgs a{out, lse, cu_q, cu_k, d->out_token_stride, d->out_head_stride, d->total_q, d->total_k, d->batch, group,
                  d->kv_heads, d->head_dim, d->causal, d->scale * kLog2e, ctx->dev_err, ctx->timeout_cycles};
     // most items that lengths summing to total_q can have: the lengths themselves are on the device
     const long long seqs = d->batch < d->total_q ? d->batch : d->total_q;

@@ -321,12 +321,42 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool b
            ((static_cast<uint32_t>(m) >> 4) << 24);
 }
 
+// Asks for the next block of this grid that has not begun: its index arrives at `response` (16 bytes, 16-byte
+// aligned) with 16 bytes announced on the mbarrier, or a refusal when none is left. After a refusal no more is asked.
+__device__ __forceinline__ void cancel_next_block(void* response, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(response)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// The answer: the block's x index, or -1.
+__device__ __forceinline__ int cancelled_block(const void* response) {
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, h;\n\t}"
+        : "=r"(ok), "=r"(x)
+        : "r"(smem_u32(response))
+        : "memory");
+    return ok ? static_cast<int>(x) : -1;
+}
+
 // Programmatic dependent launch: wait for the preceding kernel's results.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ uint32_t elect_lane0() { return (threadIdx.x & 31u) == 0; }
 
 }  // namespace tb
