@@ -58,8 +58,9 @@ template <int DCH>
 struct PromptCfg {
     static constexpr int kChunk = kRows * 128;        // one chunk of a tile: 128 rows of 128 bytes, swizzled
     static constexpr int kTile = DCH * kChunk;
-    static constexpr int kStages = DCH == 2 ? 5 : 8;  // ring of K and V blocks
-    static constexpr int kTiles = (2 + kStages) * kTile;
+    static constexpr int kStages = DCH == 2 ? 4 : 6;  // ring of K and V blocks
+    static constexpr int kStaging = 8 * 4096;         // each softmax warp's 32 result rows of 64 elements, swizzled
+    static constexpr int kTiles = (2 + kStages) * kTile + kStaging;
 };
 
 // A guarded value that is not finite is noted by its key, counted from the item's first guarded block.
@@ -202,11 +203,12 @@ __device__ __forceinline__ void weights(const float* x, uint64_t scale, uint64_t
 template <bool BF16, int DCH>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const PromptArgs a) {
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const PromptArgs a) {
     using Cfg = PromptCfg<DCH>;
     constexpr int S = Cfg::kStages;
-    extern __shared__ __align__(1024) uint8_t sq[];  // Q tiles, ring, PromptShared
+    extern __shared__ __align__(1024) uint8_t sq[];  // Q tiles, ring, staging, PromptShared
     uint8_t* ring = sq + 2 * Cfg::kTile;
+    uint8_t* staging = ring + S * Cfg::kTile;
     PromptShared& sh = *reinterpret_cast<PromptShared*>(sq + Cfg::kTiles);
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     volatile int* abort_flag = &sh.abort;
@@ -243,6 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
+        tma_prefetch_desc(&tmO);
     }
     tc_fence_before();
     __syncthreads();
@@ -626,48 +629,71 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const bool live = r < my.rows, any = sees > 0;
             // (a reference that is not finite: a score of NaN or +inf, or every score -inf)
-            const float inv = any ? (isfinite(m) ? 1.f / l : NAN) : 0.f;
+            const float inv = any ? (isfinite(m) ? __fdividef(1.f, l) : NAN) : 0.f;
             const int odd = sh.odd[k % kItems];
             const uint16_t* first = reinterpret_cast<const uint16_t*>(&sh.first[k % kItems][0][0]);
             const int rel = odd ? sees - first_guarded(tile_of(a, it, 0), tile_of(a, it, 1)) * kKeys : 0;
-            uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(it.q0 + row) * a.o_token + my.head * a.o_head;
-            for (int c = 0; c < a.head_dim; c += 16) {
-                uint32_t o[16];
+            // Each thread has a row, but the result leaves by TMA, 64 elements of the warp's 32 rows at a
+            // time through its staging buffer (stores straight from the row's thread touch 32 lines an
+            // instruction and took 6,300 cycles an item). A warp whose rows end inside the 32 stores its
+            // rows itself, so that nothing past the sequence's end is written.
+            const int warp_row = r & ~31;
+            uint4* st = reinterpret_cast<uint4*>(staging + warp * 4096);
+            const bool whole = warp_row + 32 <= my.rows;
+#pragma unroll 1
+            for (int c0 = 0; c0 < a.head_dim; c0 += 64) {
+                uint32_t o[64];
                 if (my.blocks > 0) {
-                    tmem_ld_32x32b_x16(to + c, o);
+                    tmem_ld_32x32b_x32(to + c0, *reinterpret_cast<uint32_t(*)[32]>(o));
+                    tmem_ld_32x32b_x32(to + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(o[i]));
+                    for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(o[i]));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = 0;
+                    for (int i = 0; i < 64; ++i) o[i] = 0;
                 }
                 if (odd) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
+                    for (int i = 0; i < 64; ++i) {
                         float y = __uint_as_float(o[i]);
-                        if (first[c + i] < rel) y = NAN;
-                        if (first[kKeys + c + i] < rel) y += INFINITY;
-                        if (first[2 * kKeys + c + i] < rel) y -= INFINITY;
+                        if (first[c0 + i] < rel) y = NAN;
+                        if (first[kKeys + c0 + i] < rel) y += INFINITY;
+                        if (first[2 * kKeys + c0 + i] < rel) y -= INFINITY;
                         o[i] = __float_as_uint(y);
                     }
                 }
-                uint32_t h[8];
+                uint32_t h[32];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    h[i] = any ? pack2<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
-                if (live) {
-                    *reinterpret_cast<uint4*>(out + c) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+                for (int i = 0; i < 32; ++i) h[i] = pack2<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                if (lane == 0) bulk_wait_read0();  // the buffer's last store has left
+                __syncwarp();
+#pragma unroll
+                for (int v = 0; v < 8; ++v) st[lane * 8 + (v ^ (lane & 7))] = make_uint4(h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
+                if (whole) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_3d(&tmO, st, c0, my.head, it.q0 + my.row0 + warp_row);
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(it.q0 + my.row0 + warp_row) * a.o_token + my.head * a.o_head + c0;
+                    const int v = lane & 7;
+                    for (int rr = lane >> 3; warp_row + rr < my.rows && rr < 32; rr += 4)
+                        if (c0 + 8 * v < a.head_dim) *reinterpret_cast<uint4*>(out + rr * a.o_token + 8 * v) = st[rr * 8 + (v ^ (rr & 7))];
                 }
             }
             if (a.lse != nullptr && live)
                 a.lse[static_cast<long long>(my.head) * a.total_q + it.q0 + row] =
-                    any && m != -INFINITY ? (m + log2f(l)) * kLn2 : -INFINITY;
+                    any && m != -INFINITY ? (m + __log2f(l)) * kLn2 : -INFINITY;
             tc_fence_before();
             done_with_item(k);
         }
         if (!ok) gave_up();
+        if (lane == 0) bulk_wait0();  // the warp's TMA stores are done before the CTA exits
+        __syncwarp();
     }
     __syncthreads();
     if (warp == 8) {
@@ -688,21 +714,21 @@ tb_status attention_check(const char* op, int dtype, int q_heads, int kv_heads, 
     return TB_OK;
 }
 
-// [tokens][heads][head_dim] as {head_dim, heads, tokens}, boxes of 128 tokens by 64 elements of one head.
+// [tokens][heads][head_dim] as {head_dim, heads, tokens}, boxes of some tokens by 64 elements of one head.
 static tb_status tile_map(CUtensorMap* m, const tb_attention_desc* d, const void* p, int64_t heads, int64_t tokens,
-                          int64_t token_stride, int64_t head_stride) {
+                          int64_t token_stride, int64_t head_stride, int box_tokens = kRows) {
     // the stride of a dimension of one element says nothing; the map wants a valid one
     const uint64_t head = heads > 1 ? head_stride : d->head_dim, token = tokens > 1 ? token_stride : d->head_dim;
     const uint64_t dims[3] = {static_cast<uint64_t>(d->head_dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens)};
     const uint64_t strides[2] = {head * 2, token * 2};
-    const uint32_t box[3] = {64, 1, kRows};
+    const uint32_t box[3] = {64, 1, static_cast<uint32_t>(box_tokens)};
     return encode_tiled(m, d->dtype == TB_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p,
                         dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <bool BF16, int DCH>
 static tb_status launch_prompt(tb_context* ctx, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                               const PromptArgs& a, long long grid, cudaStream_t st) {
+                               const CUtensorMap& o, const PromptArgs& a, long long grid, cudaStream_t st) {
     auto* kernel = prompt_kernel<BF16, DCH>;
     constexpr int kSmem = PromptCfg<DCH>::kTiles + static_cast<int>(sizeof(PromptShared));
     static bool ready = false;  // the attribute is per function and process-wide
@@ -725,7 +751,7 @@ static tb_status launch_prompt(tb_context* ctx, const CUtensorMap& q, const CUte
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    TB_CUDA(cudaLaunchKernelEx(&cfg, kernel, q, k, v, a));
+    TB_CUDA(cudaLaunchKernelEx(&cfg, kernel, q, k, v, o, a));
     ctx->launches++;
     return TB_OK;
 }
@@ -757,10 +783,11 @@ TB_API tb_status tb_attention(tb_context* ctx, const tb_attention_desc* d, const
         return fail(TB_ERR_INVALID_ARGUMENT, "attention: tensors must be 16-byte aligned with strides that are multiples of 8");
     // without keys nothing is loaded; the maps are made of q's first row
     const bool keys = d->total_k > 0;
-    CUtensorMap mq, mk, mv;
+    CUtensorMap mq, mk, mv, mo;
     TB_TRY(tile_map(&mq, d, q, d->q_heads, d->total_q, d->q_token_stride, d->q_head_stride));
     TB_TRY(tile_map(&mk, d, keys ? k : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->k_token_stride, d->k_head_stride));
     TB_TRY(tile_map(&mv, d, keys ? v : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->v_token_stride, d->v_head_stride));
+    TB_TRY(tile_map(&mo, d, out, d->q_heads, d->total_q, d->out_token_stride, d->out_head_stride, 32));
     const int group = d->q_heads / d->kv_heads;
     PromptArgs a{out, lse, cu_q, cu_k, d->out_token_stride, d->out_head_stride, d->total_q, d->total_k, d->batch, group,
                  d->kv_heads, d->head_dim, d->causal, d->scale * kLog2e, ctx->dev_err, ctx->timeout_cycles};
@@ -771,8 +798,8 @@ TB_API tb_status tb_attention(tb_context* ctx, const tb_attention_desc* d, const
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool wide = d->head_dim > 64;
     if (d->dtype == TB_DT_BF16)
-        return wide ? launch_prompt<true, 2>(ctx, mq, mk, mv, a, grid, st) : launch_prompt<true, 1>(ctx, mq, mk, mv, a, grid, st);
-    return wide ? launch_prompt<false, 2>(ctx, mq, mk, mv, a, grid, st) : launch_prompt<false, 1>(ctx, mq, mk, mv, a, grid, st);
+        return wide ? launch_prompt<true, 2>(ctx, mq, mk, mv, mo, a, grid, st) : launch_prompt<true, 1>(ctx, mq, mk, mv, mo, a, grid, st);
+    return wide ? launch_prompt<false, 2>(ctx, mq, mk, mv, mo, a, grid, st) : launch_prompt<false, 1>(ctx, mq, mk, mv, mo, a, grid, st);
 }
 
 }  // extern "C"
