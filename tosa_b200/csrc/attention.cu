@@ -3,29 +3,30 @@
 //   out_i = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q_i.k_j),  j over the keys that row i sees
 //
 // With t_j = scale * log2(e) * q_i.k_j the kernel keeps, per row, a reference m and
-// l = sum 2^(t_j - m), o = sum 2^(t_j - m) v_j. m follows the running maximum only when that has
-// grown by more than 8: l and o are then multiplied by 2^(m - m'). Between such steps a weight is at
-// most 2^8, far inside the range of both types, and since weights and their sum share m the result
-// does not depend on it. lse = (m + log2 l) ln 2.
+// l = sum 2^(t_j - m), o = sum 2^(t_j - m) v_j. m is the first block's maximum and stays while the weights
+// it gives are small enough: a block's maximum is not looked for, the sums of its weights (which are
+// needed anyway) tell when it has run away, and then the block is done again with its maximum and l and
+// o are multiplied by 2^(m - m'). Weights stay below 2^13, far inside the range of both types, and
+// since weights and their sum share m the result does not depend on it. lse = (m + log2 l) ln 2.
 //
 // An item is two tiles of 128 rows (two heads of one key head's group, or two row tiles of one head) that
 // walk the same blocks of 128 keys. One CTA an SM takes item after item: the grid has a block for each,
-// and a running CTA takes over blocks that have not begun, heaviest first within a sequence. 12 warps:
+// and a running CTA takes over blocks that have not begun, heaviest first within a sequence. 16 warps:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one row a thread: read the scores from tensor memory, write
-//                   the weights back to it as f16 / bf16, rescale o there when m moves, and store the
-//                   result at the item's end
+//                   the weights back to it as f16 / bf16, and rescale o there when m moves
 //   warp 8          issues the MMAs: S = Q K^T (both from shared memory), O += P V (P from tensor memory)
 //   warp 9          finds the items and loads by TMA: the Q tiles, then K and V blocks through a ring,
 //                   running ahead into the next item
 //   warps 10-11     look through the V blocks that some row sees only in part (see guard_block)
+//   warps 12-15     divide o by l and store it, while the softmax goes on with the next item
 // While one tile's softmax runs, the tensor cores work on the other tile. Tensor memory: S of both
 // tiles (128 columns each; P takes the first 64 of its S once the scores have been read) and O.
 //
 // Per tile and block the MMAs take 2 * 128 * 128 * head_dim multiply-adds (1024 cycles at head_dim 128)
 // and the 128 * 128 exponentials 1024 cycles of the special-function units. A tile's chain is softmax,
 // then O += P V, then the next S, so what counts is the softmax's length beside the other tile's MMAs:
-// part of the exponentials is computed as a polynomial on the otherwise idle FMA units, and the
-// first half of the weights is handed over while the second half is computed.
+// scores are handled in pairs where the instruction set allows, no maximum is formed (see above), and
+// the first half of the weights is handed over while the second half is computed.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -39,19 +40,18 @@ namespace tb {
 
 constexpr int kRows = 128;      // rows of a tile
 constexpr int kKeys = 128;      // keys of a block
-constexpr int kThreads = 384;
-// Registers: launched with 168 a thread (64,512); the softmax warpgroups take 208, the other one keeps 88.
-constexpr int kLaunchRegs = 168;
-constexpr int kSoftmaxRegs = 208;
-constexpr int kOtherRegs = 88;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split above the launch total");
-constexpr float kGrowth = 8.f;  // m follows the maximum when it has grown by more than this (powers of two)
+constexpr int kThreads = 512;
+// Registers: launched with 128 a thread (65,536); the two softmax warpgroups take 192, the others keep 64.
+constexpr int kLaunchRegs = 128;
+constexpr int kSoftmaxRegs = 192;
+constexpr int kOtherRegs = 64;
+static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "register split above the launch total");
+constexpr float kGrowth = 8.f;      // where the maximum is known, m follows it when it has grown by 2^8
+constexpr float kMostSum = 8192.f;  // 64 weights with a smaller sum are all below 2^13
 constexpr long long kDrainCycles = 2000000000ll;  // bound on a CTA's waits for its own copies and MMAs at its end
 constexpr int kGuards = 4;
 constexpr int kItems = 2;       // items announced at a time
-constexpr int kItemReaders = 11;  // warps that read an item: softmax, MMA, guards
-// Of every 8 pairs of exponentials this many are polynomials (see the kernel's head).
-constexpr int kPolyPairs = 3;
+constexpr int kItemReaders = 15;  // warps that read an item: softmax, MMA, guards, results
 
 // DCH: 64-element chunks of head_dim.
 template <int DCH>
@@ -59,26 +59,37 @@ struct PromptCfg {
     static constexpr int kChunk = kRows * 128;        // one chunk of a tile: 128 rows of 128 bytes, swizzled
     static constexpr int kTile = DCH * kChunk;
     static constexpr int kStages = DCH == 2 ? 4 : 6;  // ring of K and V blocks
-    static constexpr int kStaging = 8 * 4096;         // each softmax warp's 32 result rows of 64 elements, swizzled
+    static constexpr int kStaging = 4 * 4096;         // each result warp's 32 rows of 64 elements, swizzled
     static constexpr int kTiles = (2 + kStages) * kTile + kStaging;
 };
 
 // A guarded value that is not finite is noted by its key, counted from the item's first guarded block.
 constexpr uint32_t kNoKey = 0xFFFFu;
 
+// One tile's place: rows row0 .. row0 + rows - 1 of its sequence, of one head.
+struct Tile {
+    int row0, rows, head;
+    int blocks;       // blocks of keys that some row sees
+    int seen_by_all;  // keys that every row sees (the first row's)
+};
+
 struct Item {
-    int valid, q0, k0, lq, lk, sub, kv_head;  // sub: the first tile's number among (row tile, head of the group)
+    int valid, q0, k0, lq, lk, kv_head;
+    int blocks;         // the larger of the tiles' blocks
+    int first_guarded;  // the first block of keys that some row of a tile that takes it does not see whole
+    Tile tile[2];
 };
 
 struct PromptShared {
     alignas(16) uint4 response;  // of cancel_next_block
-    uint64_t q_full[2], q_empty[2], full[8], empty[8], guard[kGuards], s_full[2], p_half[2], p_full[2], o_full[2], drain;
+    uint64_t q_full[2], q_empty[2], full[8], empty[8], guard[kGuards], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], ml_full[2], half_done[2], drain;
     uint64_t item_full[kItems], item_empty[kItems], guard_done[kItems], next;
     uint32_t tmem;
     int abort;
     Item item[kItems];
     int odd[kItems];                          // some guarded value of the item is not finite
     uint32_t first[kItems][3][kKeys / 2];     // per dimension (16 bits): the first key with NaN, +inf, -inf
+    float2 ml[2][kRows];                      // m and l of each row
 };
 static_assert(sizeof(PromptShared) + PromptCfg<2>::kTiles <= 232448 && sizeof(PromptShared) + PromptCfg<1>::kTiles <= 232448,
               "shared memory above 227 KB");
@@ -95,66 +106,57 @@ struct PromptArgs {
     long long timeout_cycles;
 };
 
-// One tile's place: rows row0 .. row0 + rows - 1 of its sequence, of one head.
-struct Tile {
-    int row0, rows, head;
-    int blocks;     // blocks of keys that some row sees
-    int seen_by_all;  // keys that every row sees (the first row's)
-};
-
 __device__ __forceinline__ int visible(int causal, int row, int lq, int lk) {
     return causal ? max(0, min(lk, row + lk - lq + 1)) : lk;
 }
 
-__device__ __forceinline__ Tile tile_of(const PromptArgs& a, const Item& it, int t) {
+// Tile `sub` of a key head's group, in the order (row tile, head of the group).
+__device__ __forceinline__ Tile tile_of(const PromptArgs& a, int sub, int kv_head, int lq, int lk) {
     Tile x{0, 0, 0, 0, INT32_MAX};
-    const int sub = it.sub + t, rt = sub / a.group;
+    const int rt = sub / a.group;
     x.row0 = rt * kRows;
-    x.rows = min(kRows, it.lq - x.row0);
+    x.rows = min(kRows, lq - x.row0);
     if (x.rows <= 0) {
         x.rows = 0;
         return x;
     }
-    x.head = it.kv_head * a.group + (sub - rt * a.group);
-    x.blocks = (visible(a.causal, x.row0 + x.rows - 1, it.lq, it.lk) + kKeys - 1) / kKeys;
-    x.seen_by_all = visible(a.causal, x.row0, it.lq, it.lk);
+    x.head = kv_head * a.group + (sub - rt * a.group);
+    x.blocks = (visible(a.causal, x.row0 + x.rows - 1, lq, lk) + kKeys - 1) / kKeys;
+    x.seen_by_all = visible(a.causal, x.row0, lq, lk);
     return x;
-}
-
-// The first block of keys that some row of a tile that takes it does not see whole.
-__device__ __forceinline__ int first_guarded(const Tile& x, const Tile& y) {
-    return min(x.blocks > 0 ? x.seen_by_all / kKeys : INT32_MAX, y.blocks > 0 ? y.seen_by_all / kKeys : INT32_MAX);
 }
 
 // A weight of 0 does not take a key out of a product when the value is NaN or infinite. In a block
 // that some row sees only in part, V is therefore put in order before the MMA reads it: rows past the
 // sequence's end become zero, and values that are not finite become zero with their place noted
-// (first[]), to be added by the rows that do see them when they store their result. 64 threads, a few
-// hundred cycles that the ring's depth hides. `rel`: the block's first key counted from first_guarded.
+// (first[]), to be added by the rows that do see them when they are stored. 64 threads, some 400 cycles
+// that the ring's depth hides: x * 0 + acc in the type's own arithmetic is NaN from the first value on
+// that is not finite, so a block without one costs an instruction for two values. `rel`: the block's
+// first key counted from first_guarded.
+template <bool BF16>
+__device__ __forceinline__ uint32_t sticky(uint32_t x, uint32_t acc) {
+    uint32_t r;
+    if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
+    return r;
+}
+
 template <bool BF16, int DCH>
-__device__ void guard_block(PromptShared& sh, int slot, uint8_t* v, int live, int rel, int t) {
-    constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u;   // exponent of both halves
-    constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u;   // all ones + 1: a carry into bit 15
-    constexpr uint32_t kFrac = BF16 ? 0x7Fu : 0x3FFu;
-#pragma unroll 4
+__device__ void note_odd(PromptShared& sh, int slot, uint8_t* v, int rel, int t) {
+    constexpr uint32_t kExp = BF16 ? 0x7F80u : 0x7C00u, kFrac = BF16 ? 0x7Fu : 0x3FFu;
     for (int i = t; i < DCH * kKeys * 8; i += 64) {
         const int row = (i >> 3) & (kKeys - 1);
         uint4* p = reinterpret_cast<uint4*>(v) + i;
-        if (row >= live) {
-            *p = make_uint4(0, 0, 0, 0);
-            continue;
-        }
         const uint4 x = *p;
-        const uint32_t odd = (((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne)) & 0x80008000u;
-        if (odd == 0) continue;
         // swizzled place: 16-byte vector (i & 7) of the row holds vector (i & 7) ^ (row & 7)
         const int d0 = (i >> 10) * 64 + (((i & 7) ^ (row & 7)) << 3);
         uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint32_t h = (w[e >> 1] >> ((e & 1) * 16)) & 0xFFFFu;
-            if ((h & (kExp & 0xFFFFu)) != (kExp & 0xFFFFu)) continue;
+            const uint32_t shift = (e & 1) * 16, h = (w[e >> 1] >> shift) & 0xFFFFu;
+            if ((h & kExp) != kExp) continue;
             const int kind = (h & kFrac) ? 0 : ((h >> 15) ? 2 : 1);
-            const uint32_t key = min(static_cast<uint32_t>(rel + row), kNoKey - 1), shift = (e & 1) * 16;
+            const uint32_t key = min(static_cast<uint32_t>(rel + row), kNoKey - 1);
             uint32_t* word = &sh.first[slot][kind][(d0 + e) >> 1];
             uint32_t old = *word;
             while (((old >> shift) & 0xFFFFu) > key) {  // ends: the half only gets smaller
@@ -162,11 +164,31 @@ __device__ void guard_block(PromptShared& sh, int slot, uint8_t* v, int live, in
                 if (seen == old) break;
                 old = seen;
             }
-            w[e >> 1] &= (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+            w[e >> 1] &= ~(0xFFFFu << shift);
             sh.odd[slot] = 1;
         }
         *p = make_uint4(w[0], w[1], w[2], w[3]);
     }
+}
+
+template <bool BF16, int DCH>
+__device__ __forceinline__ void guard_block(PromptShared& sh, int slot, uint8_t* v, int live, int rel, int t) {
+    uint4* p = reinterpret_cast<uint4*>(v);
+    if (live < kKeys) {  // rows past the sequence's end
+        for (int i = t; i < DCH * kKeys * 8; i += 64)
+            if (((i >> 3) & (kKeys - 1)) >= live) p[i] = make_uint4(0, 0, 0, 0);
+    }
+    uint32_t acc[4] = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int i = t; i < DCH * kKeys * 8; i += 64) {
+        const uint4 x = p[i];
+        acc[0] = sticky<BF16>(x.x, acc[0]);
+        acc[1] = sticky<BF16>(x.y, acc[1]);
+        acc[2] = sticky<BF16>(x.z, acc[2]);
+        acc[3] = sticky<BF16>(x.w, acc[3]);
+    }
+    // a sum of zeros is zero of either sign; anything else is NaN
+    if (__any_sync(0xffffffffu, ((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7FFF7FFFu) != 0)) note_odd<BF16, DCH>(sh, slot, v, rel, t);
 }
 
 struct RingPos {
@@ -181,23 +203,33 @@ struct RingPos {
     }
 };
 
-// Weights 2^(t - base) of 64 scores as 32 packed pairs, and their sum.
-template <bool BF16, int POLY>
-__device__ __forceinline__ void weights(const float* x, uint64_t scale, uint64_t neg_base, uint64_t (&sum)[2], uint32_t (&p)[32]) {
+// Weights 2^(t - base) of 2 N scores as N packed pairs; returns their sum.
+template <bool BF16, int N>
+__device__ __forceinline__ float weights(const float* x, uint64_t scale, float base, uint32_t (&p)[N]) {
+    const uint64_t neg = pair_of(-base, -base);
+    uint64_t sum[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const uint64_t t = fma_pair(pair_of(x[2 * i], x[2 * i + 1]), scale, neg_base);
+    for (int i = 0; i < N; ++i) {
         float u, w;
-        if ((i & 7) >= 8 - POLY) {
-            exp2_poly(t, u, w);
-        } else {
-            split_pair(t, u, w);
-            u = exp2_fast(u);
-            w = exp2_fast(w);
-        }
+        split_pair(fma_pair(pair_of(x[2 * i], x[2 * i + 1]), scale, neg), u, w);
+        u = exp2_fast(u);
+        w = exp2_fast(w);
         sum[i & 1] = add_pair(sum[i & 1], pair_of(u, w));
         p[i] = pack2<BF16>(u, w);
     }
+    float s0, s1;
+    split_pair(add_pair(sum[0], sum[1]), s0, s1);
+    return s0 + s1;
+}
+
+__device__ __forceinline__ float top32(const float* x) {
+    float a = max3_nan(x[0], x[1], x[2]), b = max3_nan(x[3], x[4], x[5]);
+#pragma unroll
+    for (int i = 6; i < 30; i += 4) {
+        a = max3_nan(a, x[i], x[i + 1]);
+        b = max3_nan(b, x[i + 2], x[i + 3]);
+    }
+    return max3_nan(max_nan(a, b), x[30], x[31]);
 }
 
 template <bool BF16, int DCH>
@@ -221,6 +253,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sh.p_half[i], 4);
             mbar_init(&sh.p_full[i], 4);
             mbar_init(&sh.o_full[i], 1);
+            mbar_init(&sh.o_empty[i], 4);
+            mbar_init(&sh.ml_full[i], 4);
+            mbar_init(&sh.half_done[i], 1);
         }
         for (int i = 0; i < S; ++i) {
             mbar_init(&sh.full[i], 1);
@@ -264,18 +299,117 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     };
     // The k-th item, false at the end or when a wait gave up.
-    auto read_item = [&](int k, Item& it, bool& ok) {
+    auto next_item = [&](int k, bool& ok) {
         ok = wait(&sh.item_full[k % kItems], (k / kItems) & 1);
-        if (!ok) return false;
-        it = sh.item[k % kItems];
-        return it.valid != 0;
+        return ok && sh.item[k % kItems].valid != 0;
     };
     auto done_with_item = [&](int k) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.item_empty[k % kItems]);
     };
 
-    if (warp >= 8) {
+    if (warp >= 12) {
+        // -------------------------------------------------------------------- results
+        setmaxnreg_dec<kOtherRegs>();
+        grid_dependency_wait();
+        const int w = warp - 12, r = 32 * w + lane;
+        // Each thread has a row, but the result leaves by TMA, 64 elements of the warp's 32 rows at a
+        // time through its staging buffer (stores straight from the row's thread touch 32 lines an
+        // instruction and took 6,300 cycles an item). A warp whose rows end inside the 32 stores its
+        // rows itself, so that nothing past the sequence's end is written.
+        uint4* st = reinterpret_cast<uint4*>(staging + w * 4096);
+        uint32_t outs[2] = {0, 0}, prods[2] = {0, 0};
+        bool ok = true;
+        for (int k = 0; next_item(k, ok); ++k) {
+            const Item& it = sh.item[k % kItems];
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+                const Tile my = it.tile[t];
+                if (my.rows == 0) continue;
+                const int sees = visible(a.causal, min(my.row0 + r, my.row0 + my.rows - 1), it.lq, it.lk);
+                const uint32_t to = tmem + (static_cast<uint32_t>(w * 32) << 16) + 256 + t * 128;
+                ok = wait(&sh.ml_full[t], outs[t]++ & 1);
+                if (ok && my.blocks > 0) ok = wait(&sh.guard_done[k % kItems], (k / kItems) & 1) && wait(&sh.o_full[t], prods[t]++ & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const float2 ml = sh.ml[t][r];
+                const float m = ml.x, l = ml.y;
+                const bool any = sees > 0;
+                // (a reference that is not finite: a score of NaN or +inf, or every score -inf)
+                const float inv = any ? (isfinite(m) ? __fdividef(1.f, l) : NAN) : 0.f;
+                const int odd = sh.odd[k % kItems];
+                const uint16_t* first = reinterpret_cast<const uint16_t*>(&sh.first[k % kItems][0][0]);
+                const int rel = odd ? sees - it.first_guarded * kKeys : 0;
+                const bool whole = 32 * w + 32 <= my.rows;
+                const int token = it.q0 + my.row0 + 32 * w;
+#pragma unroll 1
+                for (int c0 = 0; c0 < a.head_dim; c0 += 64) {
+                    if (lane == 0) bulk_wait_read0();  // the buffer's last store has left
+                    __syncwarp();
+#pragma unroll 1
+                    for (int c = 0; c < 64; c += 32) {
+                        uint32_t o[32];
+                        if (my.blocks > 0) {
+                            tmem_ld_32x32b_x32(to + c0 + c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(o[i]));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = 0;
+                        }
+                        if (odd) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                float y = __uint_as_float(o[i]);
+                                const int d = c0 + c + i;
+                                if (first[d] < rel) y = NAN;
+                                if (first[kKeys + d] < rel) y += INFINITY;
+                                if (first[2 * kKeys + d] < rel) y -= INFINITY;
+                                o[i] = __float_as_uint(y);
+                            }
+                        }
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                h[i] = pack2<BF16>(__uint_as_float(o[8 * v + 2 * i]) * inv, __uint_as_float(o[8 * v + 2 * i + 1]) * inv);
+                            st[lane * 8 + ((c / 8 + v) ^ (lane & 7))] = make_uint4(h[0], h[1], h[2], h[3]);
+                        }
+                    }
+                    if (c0 + 64 >= a.head_dim) {  // O, m and l have been read
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.o_empty[t]);
+                    }
+                    if (whole) {
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_3d(&tmO, st, c0, my.head, token);
+                            bulk_commit();
+                        }
+                    } else {
+                        __syncwarp();
+                        uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(token) * a.o_token + my.head * a.o_head + c0;
+                        const int v = lane & 7;
+                        for (int rr = lane >> 3; 32 * w + rr < my.rows && rr < 32; rr += 4)
+                            if (c0 + 8 * v < a.head_dim) *reinterpret_cast<uint4*>(out + rr * a.o_token + 8 * v) = st[rr * 8 + (v ^ (rr & 7))];
+                        __syncwarp();
+                    }
+                }
+                if (a.lse != nullptr && r < my.rows)
+                    a.lse[static_cast<long long>(my.head) * a.total_q + token + lane] =
+                        any && m != -INFINITY ? (m + __log2f(l)) * kLn2 : -INFINITY;
+            }
+            if (!ok) break;
+            done_with_item(k);
+        }
+        if (!ok) gave_up();
+        if (lane == 0) bulk_wait0();  // the warp's TMA stores are done before the CTA exits
+        __syncwarp();
+    } else if (warp >= 8) {
         setmaxnreg_dec<kOtherRegs>();
         if (warp == 9) {
             // ---------------------------------------------------------------- items and loads
@@ -286,9 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             int b0 = 0;            // sequences before b0 have `before` items (items come in rising order, as a rule)
             long long before = 0;
             int block = blockIdx.x;
+            uint32_t asked = 0;
             for (int k = 0;; ++k) {
                 // items lie sequence behind sequence, ceil(row tiles * group / 2) for each
-                Item it{};
+                int valid = 0, q0s = 0, k0s = 0, lq = 0, lk = 0, sub = 0, kv_head = 0;
                 const long long want = block < 0 ? 0 : block / a.kv_heads;
                 if (want < before) before = b0 = 0;
                 while (block >= 0 && b0 < a.batch) {
@@ -313,14 +448,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const unsigned over = __ballot_sync(0xffffffffu, before + x > want);
                     if (over) {
                         const int l = __ffs(over) - 1;
-                        it.valid = 1;
-                        it.q0 = __shfl_sync(0xffffffffu, static_cast<int>(q0), l);
-                        it.k0 = __shfl_sync(0xffffffffu, static_cast<int>(k0), l);
-                        it.lq = __shfl_sync(0xffffffffu, static_cast<int>(q1), l) - it.q0;
-                        it.lk = __shfl_sync(0xffffffffu, static_cast<int>(k1), l) - it.k0;
+                        valid = 1;
+                        q0s = __shfl_sync(0xffffffffu, static_cast<int>(q0), l);
+                        k0s = __shfl_sync(0xffffffffu, static_cast<int>(k0), l);
+                        lq = __shfl_sync(0xffffffffu, static_cast<int>(q1), l) - q0s;
+                        lk = __shfl_sync(0xffffffffu, static_cast<int>(k1), l) - k0s;
                         // the last rows, which see the most keys, first
-                        it.sub = 2 * static_cast<int>(before + __shfl_sync(0xffffffffu, x, l) - 1 - want);
-                        it.kv_head = block - static_cast<int>(want) * a.kv_heads;
+                        sub = 2 * static_cast<int>(before + __shfl_sync(0xffffffffu, x, l) - 1 - want);
+                        kv_head = block - static_cast<int>(want) * a.kv_heads;
                         break;
                     }
                     before += __shfl_sync(0xffffffffu, x, 31);
@@ -334,17 +469,57 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (lane == 0) sh.odd[slot] = 0;
                 }
-                if (lane == 0) sh.item[slot] = it;
+                Item& it = sh.item[slot];
+                {
+                    const Tile x = tile_of(a, sub + (lane & 1), kv_head, lq, lk);  // lanes 0 and 1 have the two tiles
+                    const int guarded = x.blocks > 0 ? x.seen_by_all / kKeys : INT32_MAX;
+                    const int blocks = max(x.blocks, __shfl_xor_sync(0xffffffffu, x.blocks, 1));
+                    const int first = min(guarded, __shfl_xor_sync(0xffffffffu, guarded, 1));
+                    if (lane < 2) it.tile[lane] = x;
+                    if (lane == 0) {
+                        it.valid = valid;
+                        it.q0 = q0s;
+                        it.k0 = k0s;
+                        it.lq = lq;
+                        it.lk = lk;
+                        it.kv_head = kv_head;
+                        it.blocks = blocks;
+                        it.first_guarded = first;
+                    }
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.item_full[slot]);
-                if (!it.valid) break;
-                if (lane == 0) {  // the next item's block, while this one loads
-                    fence_proxy_async_smem();
-                    mbar_arrive_expect_tx(&sh.next, 16);
-                    cancel_next_block(&sh.response, &sh.next);
+                // the next item's block, while this one loads
+                auto ask = [&]() {
+                    if (lane == 0) {
+                        fence_proxy_async_smem();
+                        mbar_arrive_expect_tx(&sh.next, 16);
+                        cancel_next_block(&sh.response, &sh.next);
+                    }
+                    __syncwarp();
+                };
+                // (the answer is read even when a wait gave up: it must not arrive after the CTA's end)
+                auto answer = [&]() {
+                    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&sh.next, asked++ & 1, nullptr, drain_limit))) return false;
+                    block = cancelled_block(&sh.response);
+                    __syncwarp();
+                    return true;
+                };
+                if (!valid) {
+                    // The grid has more blocks than there are items (the host does not know the lengths). Those
+                    // past the last item are taken here, beside the end of the work; each left to run would
+                    // hold an SM for 3 us.
+                    while (block >= 0) {
+                        ask();
+                        if (!answer()) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                    break;
                 }
-                const Tile tile[2] = {tile_of(a, it, 0), tile_of(a, it, 1)};
-                const int blocks = max(tile[0].blocks, tile[1].blocks);
+                ask();
+                const int blocks = it.blocks;
                 auto load_block = [&](const CUtensorMap* m, int j) {
                     ok = wait(&sh.empty[r.s], r.ph ^ 1);
                     if (!ok) return;
@@ -352,39 +527,39 @@ __global__ void __launch_bounds__(kThreads, 1)
                         mbar_arrive_expect_tx(&sh.full[r.s], Cfg::kTile);
 #pragma unroll
                         for (int c = 0; c < DCH; ++c)
-                            tma_load_3d(ring + r.s * Cfg::kTile + c * Cfg::kChunk, m, &sh.full[r.s], 64 * c, it.kv_head, it.k0 + j * kKeys);
+                            tma_load_3d(ring + r.s * Cfg::kTile + c * Cfg::kChunk, m, &sh.full[r.s], 64 * c, kv_head, k0s + j * kKeys);
                     }
                     __syncwarp();
                     ++loads;
                     r.step<S>();
                 };
+                // Q's place is free only when the last item's last scores are through: until then its tiles come
+                // as far as L2, and the first K block goes ahead
+                if (lane < 2 * DCH && it.tile[lane / DCH].blocks)
+                    tma_prefetch_3d(&tmQ, 64 * (lane % DCH), it.tile[lane / DCH].head, q0s + it.tile[lane / DCH].row0);
+                __syncwarp();
+                if (blocks > 0) load_block(&tmK, 0);
                 for (int t = 0; t < 2 && ok; ++t) {
-                    if (tile[t].blocks == 0) continue;
+                    if (it.tile[t].blocks == 0) continue;
                     ok = wait(&sh.q_empty[t], (qn[t] & 1) ^ 1);
                     if (!ok) break;
                     if (lane == 0) {
                         mbar_arrive_expect_tx(&sh.q_full[t], Cfg::kTile);
 #pragma unroll
                         for (int c = 0; c < DCH; ++c)
-                            tma_load_3d(sq + t * Cfg::kTile + c * Cfg::kChunk, &tmQ, &sh.q_full[t], 64 * c, tile[t].head, it.q0 + tile[t].row0);
+                            tma_load_3d(sq + t * Cfg::kTile + c * Cfg::kChunk, &tmQ, &sh.q_full[t], 64 * c, it.tile[t].head, q0s + it.tile[t].row0);
                     }
                     __syncwarp();
                     ++qn[t];
-                    if (t == 0) load_block(&tmK, 0);
                 }
-                if (ok && tile[0].blocks == 0 && blocks > 0) load_block(&tmK, 0);
                 for (int j = 0; j < blocks && ok; ++j) {
                     load_block(&tmV, j);
                     if (ok && j + 1 < blocks) load_block(&tmK, j + 1);
                 }
-                // the answer is read even when a wait gave up: it must not arrive after the CTA's end
-                const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.next, k & 1, nullptr, drain_limit));
-                if (!ok || !got) {
+                if (!answer() || !ok) {
                     ok = false;
                     break;
                 }
-                block = cancelled_block(&sh.response);
-                __syncwarp();
             }
             if (!ok) gave_up();
             // every issued load lands before the CTA may exit
@@ -432,54 +607,55 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             RingPos r;                     // the K block at hand, then its V block, ...
             uint32_t n[2] = {0, 0};        // blocks of each tile so far
-            uint32_t qn[2] = {0, 0}, vn = 0;
+            uint32_t qn[2] = {0, 0}, on[2] = {0, 0}, vn = 0;  // Q tiles, results of each tile, V blocks so far
             bool ok = true;
-            Item it;
-            for (int k = 0; read_item(k, it, ok); ++k) {
+            for (int k = 0; next_item(k, ok); ++k) {
+                const Item& it = sh.item[k % kItems];
+                const int nb[2] = {it.tile[0].blocks, it.tile[1].blocks}, blocks = it.blocks;
+                const bool has[2] = {it.tile[0].rows > 0, it.tile[1].rows > 0};
                 done_with_item(k);
-                const Tile tile[2] = {tile_of(a, it, 0), tile_of(a, it, 1)};
-                const int blocks = max(tile[0].blocks, tile[1].blocks);
-                if (blocks == 0) continue;
+                if (blocks > 0) {
+                    ok = wait(&sh.full[r.s], r.ph);
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    if (ok && tile[t].blocks) {
-                        ok = wait(&sh.q_full[t], qn[t]++ & 1) && wait(&sh.full[r.s], r.ph);
+                    for (int t = 0; t < 2; ++t) {
+                        if (nb[t] == 0) continue;
+                        ok = ok && wait(&sh.q_full[t], qn[t]++ & 1);
                         if (!ok) break;
                         tc_fence_after();
                         scores(t, r.s);
-                        if (tile[t].blocks == 1) commit(&sh.q_empty[t]);
+                        if (nb[t] == 1) commit(&sh.q_empty[t]);
                     }
-                if (!ok) break;
-                commit(&sh.empty[r.s]);
-                r.step<S>();
-                for (int j = 0; j < blocks && ok; ++j, ++vn) {
+                    if (!ok) break;
+                    commit(&sh.empty[r.s]);
+                    r.step<S>();
+                }
+                for (int j = 0; j < blocks; ++j, ++vn) {
                     const RingPos v = r;
                     r.step<S>();
                     ok = wait(&sh.full[v.s], v.ph) && wait(&sh.guard[vn % kGuards], (vn / kGuards) & 1);
-                    if (!ok) break;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        if (j < tile[t].blocks) {
+                        if (j < nb[t]) {
+                            // the first product overwrites O, so the last result must have been read
+                            if (j == 0 && on[t] > 0) ok = ok && wait(&sh.o_empty[t], (on[t] - 1) & 1);
                             ok = ok && wait(&sh.p_half[t], n[t] & 1);
                             if (!ok) break;
                             tc_fence_after();
-                            //TR(40+t)
                             product(t, v.s, 0, j == 0);
+                            commit(&sh.half_done[t]);
                             ok = wait(&sh.p_full[t], n[t]++ & 1);
                             if (!ok) break;
                             tc_fence_after();
                             product(t, v.s, 1, false);
-                            //TR(42+t)
-                            if (j + 1 == tile[t].blocks) commit(&sh.o_full[t]);
+                            if (j + 1 == nb[t]) commit(&sh.o_full[t]);
                         }
                         if (t == 1) commit(&sh.empty[v.s]);
-                        if (j + 1 < tile[t].blocks) {
+                        if (j + 1 < nb[t]) {
                             ok = wait(&sh.full[r.s], r.ph);
                             if (!ok) break;
                             tc_fence_after();
                             scores(t, r.s);
-                            //TR(44+t)
-                            if (j + 2 == tile[t].blocks) commit(&sh.q_empty[t]);
+                            if (j + 2 == nb[t]) commit(&sh.q_empty[t]);
                         }
                     }
                     if (!ok) break;
@@ -489,6 +665,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 if (!ok) break;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) on[t] += has[t];
             }
             if (!ok) gave_up();
             commit(&sh.drain);
@@ -505,20 +683,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             RingPos r;
             uint32_t vn = 0;
             bool ok = true;
-            Item it;
-            for (int k = 0; read_item(k, it, ok); ++k) {
-                const Tile tile[2] = {tile_of(a, it, 0), tile_of(a, it, 1)};
-                const int blocks = max(tile[0].blocks, tile[1].blocks);
-                const int from = first_guarded(tile[0], tile[1]);
+            for (int k = 0; next_item(k, ok); ++k) {
+                const Item& it = sh.item[k % kItems];
+                const int blocks = it.blocks, from = it.first_guarded, lk = it.lk;
+                const int nb0 = it.tile[0].blocks, nb1 = it.tile[1].blocks, seen0 = it.tile[0].seen_by_all, seen1 = it.tile[1].seen_by_all;
                 for (int j = 0; j < blocks; ++j, ++vn) {
                     r.step<S>();  // past the K block
                     ok = wait(&sh.full[r.s], r.ph);
                     if (!ok) break;
                     // a tile that does not reach this block has no say in it
-                    const int seen = min(j < tile[0].blocks ? tile[0].seen_by_all : INT32_MAX,
-                                         j < tile[1].blocks ? tile[1].seen_by_all : INT32_MAX);
+                    const int seen = min(j < nb0 ? seen0 : INT32_MAX, j < nb1 ? seen1 : INT32_MAX);
                     if (seen < (j + 1) * kKeys) {
-                        guard_block<BF16, DCH>(sh, k % kItems, ring + r.s * Cfg::kTile, it.lk - j * kKeys, (j - from) * kKeys, threadIdx.x - 320);
+                        guard_block<BF16, DCH>(sh, k % kItems, ring + r.s * Cfg::kTile, lk - j * kKeys, (j - from) * kKeys, threadIdx.x - 320);
                         fence_proxy_async_smem();
                     }
                     __syncwarp();
@@ -535,18 +711,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // -------------------------------------------------------------------- softmax
         setmaxnreg_inc<kSoftmaxRegs>();
-        grid_dependency_wait();
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * 128;
         const uint32_t to = ts + 256;  // O
         const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2);
         uint32_t n = 0, outs = 0;  // blocks and results so far
         bool ok = true;
-        Item it;
-        for (int k = 0; read_item(k, it, ok); ++k) {
-            const Tile my = tile_of(a, it, t);
-            const int row = my.row0 + r;
-            const int sees = r < my.rows ? visible(a.causal, row, it.lq, it.lk) : it.lk;
+        for (int k = 0; next_item(k, ok); ++k) {
+            const Item& it = sh.item[k % kItems];
+            const Tile my = it.tile[t];
+            // keys that this thread's row sees, and the first and the last row of the warp (rows past the
+            // tile's end count as its last)
+            const int last = my.row0 + my.rows - 1;
+            const int sees = visible(a.causal, min(my.row0 + r, last), it.lq, it.lk);
+            const int lo = __shfl_sync(0xffffffffu, sees, 0), hi = __shfl_sync(0xffffffffu, sees, 31);
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < my.blocks; ++j, ++n) {
                 ok = wait(&sh.s_full[t], n & 1);
@@ -563,137 +741,105 @@ __global__ void __launch_bounds__(kThreads, 1)
                     asm volatile("" : "+r"(s[i]));
                     x[i] = __uint_as_float(s[i]);
                 }
-                const bool part = my.seen_by_all < (j + 1) * kKeys;  // some row does not see the whole block
-                if (part) {
-                    const int seen = sees - j * kKeys;
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) x[i] = i < seen ? x[i] : -INFINITY;
-                }
                 //TR(8+warp)
-                float top[4];
+                const int lo_j = lo - j * kKeys, hi_j = hi - j * kKeys;
+                // O and l to a new reference. (O holds every product so far: S was committed after them.)
+                auto rescale = [&](float to_m) {
+                    const float f = to_m == m ? 1.f : exp2_fast(m - to_m);
+                    m = to_m;
+                    l *= f;
+#pragma unroll 1
+                    for (int c = 0; c < a.head_dim; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld_32x32b_x16(to + c, o);
+                        tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    top[c] = x[32 * c];
-#pragma unroll
-                    for (int i = 1; i < 31; i += 2) top[c] = max3_nan(top[c], x[32 * c + i], x[32 * c + i + 1]);
-                    top[c] = max_nan(top[c], x[32 * c + 31]);
-                }
-                // a NaN among the scores becomes the row's reference and with it the whole row
-                const float m1 = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * a.scale_log2;
-                const bool grow = !(m1 <= m + kGrowth);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float mm = grow ? m1 : m;
-                    if (j > 0) {
-                        const float f = grow ? exp2_fast(m - mm) : 1.f;
-                        l *= f;
-                        for (int c = 0; c < a.head_dim; c += 16) {
-                            uint32_t o[16];
-                            tmem_ld_32x32b_x16(to + c, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                asm volatile("" : "+r"(o[i]));
-                                o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            }
-                            tmem_st_32x32b_x16(to + c, o);
+                        for (int i = 0; i < 16; ++i) {
+                            asm volatile("" : "+r"(o[i]));
+                            o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
                         }
+                        tmem_st_32x32b_x16(to + c, o);
                     }
-                    m = mm;
-                }
-                const float base = m == -INFINITY ? 0.f : m;
-                //TR(16+warp)
-                const uint64_t neg = pair_of(-base, -base);
-                uint64_t sum[2] = {0, 0};
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t p[32];
-                    // keys that are not seen get a weight of exactly 0 from the special-function unit
-                    if (part) weights<BF16, 0>(x + 64 * c, scale2, neg, sum, p);
-                    else weights<BF16, kPolyPairs>(x + 64 * c, scale2, neg, sum, p);
-                    tmem_st_32x32b_x32(ts + 32 * c, p);
+                };
+                auto hand_over = [&](uint64_t* bar) {
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(c == 0 ? &sh.p_half[t] : &sh.p_full[t]);
+                    if (lane == 0) mbar_arrive(bar);
+                };
+                bool done = false;
+                if (lo_j >= kKeys) {
+                    if (j == 0) m = max_nan(max_nan(top32(x), top32(x + 32)), max_nan(top32(x + 64), top32(x + 96))) * a.scale_log2;
+                    uint32_t p[32];
+                    const float s0 = weights<BF16, 32>(x, scale2, m, p);
+                    // (also when m is not a number yet: -inf - -inf)
+                    if (!__any_sync(0xffffffffu, !(s0 < kMostSum) || m == -INFINITY)) {
+                        tmem_st_32x32b_x32(ts, p);
+                        hand_over(&sh.p_half[t]);
+                        l += s0;
+                        float s1 = weights<BF16, 32>(x + 64, scale2, m, p);
+                        const bool ran = !(s1 < kMostSum);
+                        if (__any_sync(0xffffffffu, ran)) {
+                            // the first half's product must be through before O is rescaled
+                            ok = wait(&sh.half_done[t], n & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            rescale(ran ? max_nan(m, max_nan(top32(x + 64), top32(x + 96)) * a.scale_log2) : m);
+                            s1 = weights<BF16, 32>(x + 64, scale2, m, p);
+                        }
+                        tmem_st_32x32b_x32(ts + 32, p);
+                        hand_over(&sh.p_full[t]);
+                        l += s1;
+                        done = true;
+                    }
                 }
-                //TR(24+warp)
-                float s0, s1;
-                split_pair(add_pair(sum[0], sum[1]), s0, s1);
-                l += s0 + s1;
+                if (!done) {
+                    // Chunks of 32 keys: seen by all of the warp's rows, by some, or by none.
+                    const int seen = sees - j * kKeys;
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (32 * c >= hi_j) continue;
+                        if (32 * (c + 1) > lo_j) {
+#pragma unroll
+                            for (int i = 32 * c; i < 32 * c + 32; ++i) x[i] = i < seen ? x[i] : -INFINITY;
+                        }
+                        top = max_nan(top, top32(x + 32 * c));
+                    }
+                    // a NaN among the scores becomes the row's reference and with it the whole row
+                    top *= a.scale_log2;
+                    const bool grow = !(top <= m + kGrowth);
+                    if (j == 0) m = top;
+                    else if (__any_sync(0xffffffffu, grow)) rescale(grow ? top : m);
+                    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t p[16];
+                        if (32 * c < hi_j) {
+                            l += weights<BF16, 16>(x + 32 * c, scale2, base, p);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) p[i] = 0;
+                        }
+                        tmem_st_32x32b_x16(ts + 16 * c, p);
+                        if (c == 1) hand_over(&sh.p_half[t]);
+                    }
+                    hand_over(&sh.p_full[t]);
+                }
                 //TR(32+warp)
             }
             if (!ok) break;
-            ok = wait(&sh.guard_done[k % kItems], (k / kItems) & 1);
-            if (ok && my.blocks > 0) ok = wait(&sh.o_full[t], outs++ & 1);
-            if (!ok) break;
-            tc_fence_after();
-            const bool live = r < my.rows, any = sees > 0;
-            // (a reference that is not finite: a score of NaN or +inf, or every score -inf)
-            const float inv = any ? (isfinite(m) ? __fdividef(1.f, l) : NAN) : 0.f;
-            const int odd = sh.odd[k % kItems];
-            const uint16_t* first = reinterpret_cast<const uint16_t*>(&sh.first[k % kItems][0][0]);
-            const int rel = odd ? sees - first_guarded(tile_of(a, it, 0), tile_of(a, it, 1)) * kKeys : 0;
-            // Each thread has a row, but the result leaves by TMA, 64 elements of the warp's 32 rows at a
-            // time through its staging buffer (stores straight from the row's thread touch 32 lines an
-            // instruction and took 6,300 cycles an item). A warp whose rows end inside the 32 stores its
-            // rows itself, so that nothing past the sequence's end is written.
-            const int warp_row = r & ~31;
-            uint4* st = reinterpret_cast<uint4*>(staging + warp * 4096);
-            const bool whole = warp_row + 32 <= my.rows;
-#pragma unroll 1
-            for (int c0 = 0; c0 < a.head_dim; c0 += 64) {
-                uint32_t o[64];
-                if (my.blocks > 0) {
-                    tmem_ld_32x32b_x32(to + c0, *reinterpret_cast<uint32_t(*)[32]>(o));
-                    tmem_ld_32x32b_x32(to + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(o[i]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) o[i] = 0;
-                }
-                if (odd) {
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        float y = __uint_as_float(o[i]);
-                        if (first[c0 + i] < rel) y = NAN;
-                        if (first[kKeys + c0 + i] < rel) y += INFINITY;
-                        if (first[2 * kKeys + c0 + i] < rel) y -= INFINITY;
-                        o[i] = __float_as_uint(y);
-                    }
-                }
-                uint32_t h[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) h[i] = pack2<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-                if (lane == 0) bulk_wait_read0();  // the buffer's last store has left
+            if (my.rows > 0) {
+                if (outs > 0) ok = wait(&sh.o_empty[t], (outs - 1) & 1);  // the last m and l have been read
+                if (!ok) break;
+                ++outs;
+                sh.ml[t][r] = make_float2(m, l);
                 __syncwarp();
-#pragma unroll
-                for (int v = 0; v < 8; ++v) st[lane * 8 + (v ^ (lane & 7))] = make_uint4(h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
-                if (whole) {
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_3d(&tmO, st, c0, my.head, it.q0 + my.row0 + warp_row);
-                        bulk_commit();
-                    }
-                } else {
-                    __syncwarp();
-                    uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(it.q0 + my.row0 + warp_row) * a.o_token + my.head * a.o_head + c0;
-                    const int v = lane & 7;
-                    for (int rr = lane >> 3; warp_row + rr < my.rows && rr < 32; rr += 4)
-                        if (c0 + 8 * v < a.head_dim) *reinterpret_cast<uint4*>(out + rr * a.o_token + 8 * v) = st[rr * 8 + (v ^ (rr & 7))];
-                }
+                if (lane == 0) mbar_arrive(&sh.ml_full[t]);
             }
-            if (a.lse != nullptr && live)
-                a.lse[static_cast<long long>(my.head) * a.total_q + it.q0 + row] =
-                    any && m != -INFINITY ? (m + __log2f(l)) * kLn2 : -INFINITY;
-            tc_fence_before();
             done_with_item(k);
         }
         if (!ok) gave_up();
-        if (lane == 0) bulk_wait0();  // the warp's TMA stores are done before the CTA exits
-        __syncwarp();
     }
     __syncthreads();
     if (warp == 8) {
@@ -793,7 +939,8 @@ TB_API tb_status tb_attention(tb_context* ctx, const tb_attention_desc* d, const
                  d->kv_heads, d->head_dim, d->causal, d->scale * kLog2e, ctx->dev_err, ctx->timeout_cycles};
     // most items that lengths summing to total_q can have: the lengths themselves are on the device
     const long long seqs = d->batch < d->total_q ? d->batch : d->total_q;
-    const long long grid = ((d->total_q / kRows + seqs) * group / 2 + seqs) * d->kv_heads;
+    const long long tiles = (d->total_q - seqs) / kRows + seqs;
+    const long long grid = (group % 2 ? (tiles * group + seqs) / 2 : tiles * (group / 2)) * d->kv_heads;
     if (grid > INT32_MAX) return fail(TB_ERR_NOT_ACCELERATED, "attention: more than 2^31 tiles");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool wide = d->head_dim > 64;

@@ -60,28 +60,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// 2^x of a pair for x <= 127 without the special-function unit: x = n + f with n the nearest integer (left
-// in the low bits by adding 1.5 * 2^23) and |f| <= 1/2, 2^f by the polynomial of degree 4 whose largest
-// relative error there is least (2.6e-6; found by Remez exchange), n added to its exponent. x below -125
-// gives 2^-125.
-__device__ __forceinline__ void exp2_poly(uint64_t x, float& a, float& b) {
-    float x0, x1;
-    split_pair(x, x0, x1);
-    x = pair_of(max_nan(x0, -125.f), max_nan(x1, -125.f));
-    const float kMagic = 12582912.f;
-    const uint64_t r = add_pair(x, pair_of(kMagic, kMagic));
-    const uint64_t f = fma_pair(add_pair(r, pair_of(-kMagic, -kMagic)), pair_of(-1.f, -1.f), x);
-    uint64_t p = fma_pair(f, pair_of(0x1.3997d6p-7f, 0x1.3997d6p-7f), pair_of(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-    p = fma_pair(p, f, pair_of(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    p = fma_pair(p, f, pair_of(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    p = fma_pair(p, f, pair_of(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-    float r0, r1, p0, p1;
-    split_pair(r, r0, r1);
-    split_pair(p, p0, p1);
-    a = __uint_as_float((__float_as_uint(r0) << 23) + __float_as_uint(p0));
-    b = __uint_as_float((__float_as_uint(r1) << 23) + __float_as_uint(p1));
-}
-
 // head_dim, heads, scale: the conditions that both attention operators share.
 tb_status attention_check(const char* op, int dtype, int q_heads, int kv_heads, int head_dim, float scale);
 
