@@ -3,8 +3,9 @@
 //   out_i = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q_i.k_j),  j over the keys that row i sees
 //
 // With t_j = scale * log2(e) * q_i.k_j the kernel keeps, per row, a reference m and
-// l = sum 2^(t_j - m), o = sum 2^(t_j - m) v_j. m is the first block's maximum and stays while the weights
-// it gives are small enough: a block's maximum is not looked for, the sums of its weights (which are
+// l = sum 2^(t_j - m), o = sum 2^(t_j - m) v_j. m is the maximum of the first 32 keys (of the first
+// block, where the row does not see all of it) and stays while the weights it gives are small enough: a
+// block's maximum is not looked for, the sums of its weights (which are
 // needed anyway) tell when it has run away, and then the block is done again with its maximum and l and
 // o are multiplied by 2^(m - m'). Weights stay below 2^13, far inside the range of both types, and
 // since weights and their sum share m the result does not depend on it. lse = (m + log2 l) ln 2.
@@ -417,48 +418,65 @@ __global__ void __launch_bounds__(kThreads, 1)
             RingPos r;
             uint32_t loads = 0, qn[2] = {0, 0};
             bool ok = true;
-            int b0 = 0;            // sequences before b0 have `before` items (items come in rising order, as a rule)
-            long long before = 0;
+            // Items lie sequence behind sequence, ceil(row tiles * group / 2) for each; sequences whose rows see
+            // many keys first (by the power of two of their blocks), so that no long item begins late.
+            int level = 32, b0 = a.batch;  // sequences of this level before b0, and of higher levels, have
+            long long before = 0;          // `before` items (items come in rising order, as a rule)
             int block = blockIdx.x;
             uint32_t asked = 0;
+            struct Seq { int q0, k0, lq, lk, level; };
+            auto look_at = [&](int b) {
+                Seq x{0, 0, 0, 0, -1};
+                if (b < a.batch) {
+                    const int q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+                    // (sequences out of range are reported by the first block's warp 10)
+                    if (q0 >= 0 && q1 > q0 && q1 <= a.total_q && k0 >= 0 && k1 >= k0 && k1 <= a.total_k) {
+                        x = Seq{q0, k0, q1 - q0, k1 - k0, 0};
+                        x.level = 31 - __clz(visible(a.causal, x.lq - 1, x.lq, x.lk) / kKeys + 1);
+                    }
+                }
+                return x;
+            };
             for (int k = 0;; ++k) {
-                // items lie sequence behind sequence, ceil(row tiles * group / 2) for each
                 int valid = 0, q0s = 0, k0s = 0, lq = 0, lk = 0, sub = 0, kv_head = 0;
                 const long long want = block < 0 ? 0 : block / a.kv_heads;
-                if (want < before) before = b0 = 0;
-                while (block >= 0 && b0 < a.batch) {
-                    const int b = b0 + lane;
-                    int items = 0;
-                    long long q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-                    if (b < a.batch) {
-                        q0 = a.cu_q[b];
-                        q1 = a.cu_q[b + 1];
-                        k0 = a.cu_k[b];
-                        k1 = a.cu_k[b + 1];
-                        // (sequences out of range are reported by the first block's warp 10)
-                        if (!(q0 < 0 || q1 < q0 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k))
-                            items = static_cast<int>(((q1 - q0 + kRows - 1) / kRows * a.group + 1) >> 1);
+                if (want < before) {
+                    level = 32;
+                    b0 = a.batch;
+                    before = 0;
+                }
+                while (block >= 0) {
+                    if (b0 >= a.batch) {  // the next lower level that occurs
+                        int top = -1;
+                        for (int b = lane; b < a.batch; b += 32) {
+                            const int l = look_at(b).level;
+                            if (l < level) top = max(top, l);
+                        }
+                        level = __reduce_max_sync(0xffffffffu, top);
+                        if (level < 0) break;
+                        b0 = 0;
                     }
-                    int x = items;
+                    const Seq x = look_at(b0 + lane);
+                    int n = x.level == level ? ((x.lq + kRows - 1) / kRows * a.group + 1) >> 1 : 0;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
-                        const int y = __shfl_up_sync(0xffffffffu, x, o);
-                        if (lane >= o) x += y;
+                        const int y = __shfl_up_sync(0xffffffffu, n, o);
+                        if (lane >= o) n += y;
                     }
-                    const unsigned over = __ballot_sync(0xffffffffu, before + x > want);
+                    const unsigned over = __ballot_sync(0xffffffffu, before + n > want);
                     if (over) {
                         const int l = __ffs(over) - 1;
                         valid = 1;
-                        q0s = __shfl_sync(0xffffffffu, static_cast<int>(q0), l);
-                        k0s = __shfl_sync(0xffffffffu, static_cast<int>(k0), l);
-                        lq = __shfl_sync(0xffffffffu, static_cast<int>(q1), l) - q0s;
-                        lk = __shfl_sync(0xffffffffu, static_cast<int>(k1), l) - k0s;
+                        q0s = __shfl_sync(0xffffffffu, x.q0, l);
+                        k0s = __shfl_sync(0xffffffffu, x.k0, l);
+                        lq = __shfl_sync(0xffffffffu, x.lq, l);
+                        lk = __shfl_sync(0xffffffffu, x.lk, l);
                         // the last rows, which see the most keys, first
-                        sub = 2 * static_cast<int>(before + __shfl_sync(0xffffffffu, x, l) - 1 - want);
+                        sub = 2 * static_cast<int>(before + __shfl_sync(0xffffffffu, n, l) - 1 - want);
                         kv_head = block - static_cast<int>(want) * a.kv_heads;
                         break;
                     }
-                    before += __shfl_sync(0xffffffffu, x, 31);
+                    before += __shfl_sync(0xffffffffu, n, 31);
                     b0 += 32;
                 }
                 const int slot = k % kItems;
@@ -769,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 bool done = false;
                 if (lo_j >= kKeys) {
-                    if (j == 0) m = max_nan(max_nan(top32(x), top32(x + 32)), max_nan(top32(x + 64), top32(x + 96))) * a.scale_log2;
+                    if (j == 0) m = top32(x) * a.scale_log2;
                     uint32_t p[32];
                     const float s0 = weights<BF16, 32>(x, scale2, m, p);
                     // (also when m is not a number yet: -inf - -inf)
