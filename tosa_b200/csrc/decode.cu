@@ -2,10 +2,10 @@
 //
 // The formula is attention.cu's with one row a sequence. Every key and value is read once and used
 // for the group's query heads only, so the kernel is bound by memory bandwidth: its work is cut so that
-// every SM streams the same amount, and the arithmetic (mma.sync on 16 query rows, most of them
-// padding) only has to keep up.
+// every SM streams the same amount, and the arithmetic only has to keep up. Keys and dimensions take
+// the long side of mma.sync's 16 x 8 x 16 and the query rows the short one, so at most 7 rows are padding.
 //
-// Cut: a unit is one sequence, key head and at most 16 of its query heads; its keys come in tiles of 64
+// Cut: a unit is one sequence, key head and at most 8 (for groups above 8: 16) of its query heads; its keys come in tiles of 64
 // tokens. The tiles of all units in a row are divided evenly over the CTAs (two on each SM), so a CTA
 // takes the end of one unit, some whole units and the beginning of another. A unit that lies in one CTA
 // is finished there. Of a unit that several CTAs share, each leaves its unscaled sum, maximum and sum of
@@ -14,9 +14,12 @@
 // whole batch.) Nobody waits for another CTA.
 //
 // A CTA: warp 4 looks the pages up and loads K and V tiles by TMA (boxes as high as the greatest common
-// divisor of 64 and the page size, so that a box never crosses a page) and the query rows, three tiles
-// ahead; warps 0-3 take 16 of a tile's 64 keys each for S = Q K^T, share the maximum and the weights through
-// shared memory, and take a quarter of head_dim each for O += P V. Two barriers a tile.
+// divisor of 64 and the page size, so that a box never crosses a page) and the query rows, as many tiles
+// ahead as the ring holds (96 KB). Warps 0-3 take 16 of a tile's 64 keys each for S^T = K Q^T, share the
+// maximum and the weights through shared memory, and take a quarter of head_dim each for
+// O^T += V^T P^T: two barriers a tile, and nothing to join among the warps when the CTA leaves a unit
+// (warps with a maximum and a result of their own need no barriers, but joining them took 2000 cycles
+// a unit and made short contexts and few rows slower).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -30,19 +33,19 @@
 namespace tb {
 
 constexpr int kTokens = 64;                    // keys of a tile
-constexpr int kUnitRows = 16;                  // query rows of a unit
+constexpr int kUnitRows = 16;                  // query rows of a unit at most
 constexpr int kConsumers = 128;
 constexpr int kDecodeThreads = kConsumers + 32;
-constexpr int kDecodeStages = 3;
 constexpr int kQPitch = 272;                   // bytes from one query row to the next: 8 rows hit 8 bank groups
-constexpr int kPPitch = 144;                   // the same for the weights
+constexpr int kPPitch = 144;                   // bytes of one row of weights: 8 rows hit 8 bank groups
 constexpr long long kDecodeDrain = 2000000000ll;  // bound on a CTA's waits for its own copies at its end
 
 template <int DCH>
 struct DecodeCfg {
     static constexpr int kTensor = DCH * kTokens * 128;  // K or V of a tile, 64-element chunks of 128-byte rows, swizzled
     static constexpr int kStage = 2 * kTensor;
-    static constexpr int kSmem = 1024 + kDecodeStages * kStage + 2 * kUnitRows * kQPitch + kUnitRows * kPPitch;
+    static constexpr int kStages = DCH == 2 ? 3 : 6;
+    static constexpr int kSmem = 1024 + kStages * kStage + kUnitRows * kQPitch + kUnitRows * kPPitch;
 };
 
 struct DecodeArgs {
@@ -62,81 +65,84 @@ struct DecodeArgs {
 };
 
 struct DecodeShared {
-    uint64_t full[kDecodeStages], empty[kDecodeStages], q_full[2], q_empty[2];
+    uint64_t full[6], empty[6], q_full[4], q_empty[4];
     float top[4][kUnitRows], sum[4][kUnitRows];
-    long long scan[kDecodeThreads / 32];
-    long long start_before;    // tiles before the start's row
-    int start_row;
     int abort, last;
 };
 
-// Tiles of one row's units, 0 when the row is refused. A row without tokens has one empty tile.
-__device__ __forceinline__ int row_tiles(const DecodeArgs& a, int i, int& slot, int& len, uint32_t& err) {
-    slot = a.slots[i];
-    if (slot < 0 || slot >= a.max_seqs) {
-        err |= DEV_ERR_INDEX;
-        return 0;
-    }
-    len = a.lengths[slot];
-    if (len < 0 || static_cast<long long>(len) > static_cast<long long>(a.max_pages) * a.page_size) {
-        err |= DEV_ERR_INDEX;
-        return 0;
-    }
-    return max(1, (len + kTokens - 1) / kTokens);
+// Tiles of a row's units, 0 when the row is refused. A row without tokens has one empty tile.
+__device__ __forceinline__ bool row_ok(const DecodeArgs& a, int slot, int len) {
+    return slot >= 0 && slot < a.max_seqs && len >= 0 && static_cast<long long>(len) <= static_cast<long long>(a.max_pages) * a.page_size;
+}
+__device__ __forceinline__ int row_tiles(int len) { return max(1, (len + kTokens - 1) / kTokens); }
+
+// a / b for a >= 0, b > 0; nearly always of 32 bits, where a division is ten times as fast.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
 }
 
 // This CTA's tiles, segment by segment: tiles [t0, t1) of one unit.
 struct Walk {
-    long long x, end, rem;   // next tile, end of the CTA's tiles, tiles of row i before x
-    int i, nt, len, slot;
+    long long x, end;        // the next tile and the end of the CTA's
+    int i, nt, len, slot;    // row, tiles of each of its units, tokens
     int unit, t0, t1;
     long long unit_start;    // the unit's first tile
-    __device__ void begin(const DecodeArgs& a, long long x0, long long x1, int row, long long before) {
+    // From tile x0, which is `rem` tiles into row i's units.
+    __device__ void begin(long long x0, long long x1, int row, int row_slot, int row_len, long long rem) {
         x = x0;
         end = x1;
         i = row;
-        rem = x0 - before;
-        uint32_t e = 0;
-        nt = x < end ? row_tiles(a, i, slot, len, e) : 0;
+        slot = row_slot;
+        len = row_len;
+        nt = row_tiles(len);
+        unit = static_cast<int>(quotient(rem, nt));
+        t1 = static_cast<int>(rem - static_cast<long long>(unit) * nt);
     }
     __device__ bool next(const DecodeArgs& a) {
         if (x >= end) return false;
-        const int units = a.kv_heads * a.chunks;
-        while (rem >= static_cast<long long>(nt) * units) {
-            uint32_t e = 0;
-            if (++i >= a.n) return false;  // (x < end: a row with tiles follows, unless lengths change meanwhile)
-            nt = row_tiles(a, i, slot, len, e);
-            rem = 0;
+        if (t1 == nt) {
+            t1 = 0;
+            ++unit;
         }
-        unit = static_cast<int>(rem / nt);
-        t0 = static_cast<int>(rem - static_cast<long long>(unit) * nt);
+        t0 = t1;
+        if (unit == a.kv_heads * a.chunks) {
+            unit = 0;
+            do {
+                if (++i >= a.n) return false;  // (x < end: a row with tiles follows, unless lengths change meanwhile)
+                slot = a.slots[i];
+                len = a.lengths[min(max(slot, 0), a.max_seqs - 1)];
+            } while (!row_ok(a, slot, len));
+            nt = row_tiles(len);
+        }
         t1 = static_cast<int>(min(static_cast<long long>(nt), t0 + (end - x)));
         unit_start = x - t0;
         x += t1 - t0;
-        rem += t1 - t0;
         return true;
     }
 };
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-template <bool BF16, int DCH>
+// NT: query rows of a unit / 8.
+template <bool BF16, int DCH, int NT>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
     decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a) {
     using Cfg = DecodeCfg<DCH>;
+    constexpr int S = Cfg::kStages;
     extern __shared__ uint8_t raw[];
     __shared__ DecodeShared sh;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* sq = ring + kDecodeStages * Cfg::kStage;
-    uint8_t* sp = sq + 2 * kUnitRows * kQPitch;
+    uint8_t* sq = ring + S * Cfg::kStage;
+    uint8_t* sp = sq + kUnitRows * kQPitch;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &sh.abort;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kDecodeStages; ++i) {
+        for (int i = 0; i < S; ++i) {
             mbar_init(&sh.full[i], 1);
             mbar_init(&sh.empty[i], 4);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&sh.q_full[i], 1);
             mbar_init(&sh.q_empty[i], 4);
         }
@@ -145,76 +151,90 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
     }
+    if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
 
-    // All tiles, this CTA's part of them, and the row where it begins. Four rows a thread and pass.
+    __syncthreads();  // the barriers are made
+    // All tiles, this CTA's part of them, and the row where it begins: each warp for itself, four rows a
+    // lane and pass, so that no barrier stands before the first load.
     const int units = a.kv_heads * a.chunks;
     uint32_t err = 0;
-    auto pass = [&](int i0, long long (&w)[4]) {
-        long long s = 0;
+    int slot[4], len[4];
+    long long w[4];
+    auto pass = [&](int i0) {  // tiles of the lane's four rows, before it (exclusive) and of the warp's 128
+        const int i = i0 + 4 * lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) slot[j] = i + j < a.n ? a.slots[i + j] : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) len[j] = a.lengths[min(max(slot[j], 0), a.max_seqs - 1)];
+        long long sum = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int i = i0 + 4 * static_cast<int>(threadIdx.x) + j;
-            int slot, len;
-            w[j] = i < a.n ? static_cast<long long>(row_tiles(a, i, slot, len, err)) * units : 0;
-            s += w[j];
+            const bool ok = row_ok(a, slot[j], len[j]);
+            w[j] = i + j < a.n && ok ? static_cast<long long>(row_tiles(len[j])) * units : 0;
+            if (i + j < a.n && !ok) err |= DEV_ERR_INDEX;
+            sum += w[j];
         }
-        return s;
-    };
-    auto block_prefix = [&](long long v, long long& total) {  // exclusive, over the block
-        long long p = v;
+        long long p = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, p, o);
             if (lane >= o) p += y;
         }
-        __syncthreads();
-        if (lane == 31) sh.scan[warp] = p;
-        __syncthreads();
-        long long pre = 0;
-        total = 0;
-#pragma unroll
-        for (int k = 0; k < kDecodeThreads / 32; ++k) {
-            if (k < warp) pre += sh.scan[k];
-            total += sh.scan[k];
-        }
-        return pre + p - v;
+        return longlong2{p - sum, __shfl_sync(0xffffffffu, p, 31)};
     };
-    constexpr int kStep = 4 * kDecodeThreads;
-    long long w[4], total = 0, sum = 0, pre = 0;
+    constexpr int kStep = 128;
+    longlong2 part{0, 0};
+    long long total = 0;
     for (int i0 = 0; i0 < a.n; i0 += kStep) {
-        sum = pass(i0, w);
-        long long t;
-        pre = block_prefix(sum, t);
-        total += t;
+        part = pass(i0);
+        total += part.y;
     }
     if (err != 0 && blockIdx.x == 0) atomicOr(a.err, err);
+    // one tile a CTA is enough: 2 and 3 at least made one user's 333 tokens 6.9 and 7.6 us instead of 6.4
     const long long ctas = min(static_cast<long long>(gridDim.x), total);
     if (blockIdx.x >= ctas) return;
-    auto bound = [&](long long c) { return c * total / ctas; };
-    const long long x0 = bound(blockIdx.x), x1 = bound(blockIdx.x + 1);
-    long long before = 0;
-    for (int i0 = 0; i0 < a.n; i0 += kStep) {
-        if (a.n > kStep) {  // (otherwise the first pass' values are still there)
-            sum = pass(i0, w);
-            long long t;
-            pre = block_prefix(sum, t) + before;
-            before += t;
-        }
-        long long at = pre;
+    // the first `longer` CTAs take share + 1 tiles, the others share
+    const long long share = quotient(total, ctas), longer = total - share * ctas;
+    auto bound = [&](long long c) { return c * share + min(c, longer); };
+    auto cta_of = [&](long long x) {
+        const long long split = longer * (share + 1);
+        return x < split ? quotient(x, share + 1) : longer + quotient(x - split, share);
+    };
+    const long long x0 = bound(blockIdx.x), x1 = bound(blockIdx.x + 1ll);
+    Walk walk;
+    {
+        long long before = 0;
+        for (int i0 = 0; i0 < a.n; i0 += kStep) {
+            if (a.n > kStep) part = pass(i0);  // (otherwise the first pass' values are still there)
+            if (x0 < before + part.y) {
+                long long at = before + part.x;
+                int j0 = 0;
+                bool here = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (at <= x0 && x0 < at + w[j]) {
-                sh.start_row = i0 + 4 * static_cast<int>(threadIdx.x) + j;
-                sh.start_before = at;
+                for (int j = 0; j < 4; ++j) {
+                    if (!here) {
+                        if (at <= x0 && x0 < at + w[j]) {
+                            here = true;
+                            j0 = j;
+                        } else {
+                            at += w[j];
+                        }
+                    }
+                }
+                const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+                const int row_slot = j0 == 0 ? slot[0] : (j0 == 1 ? slot[1] : (j0 == 2 ? slot[2] : slot[3]));
+                const int row_len = j0 == 0 ? len[0] : (j0 == 1 ? len[1] : (j0 == 2 ? len[2] : len[3]));
+                walk.begin(x0, x1, __shfl_sync(0xffffffffu, i0 + 4 * lane + j0, from), __shfl_sync(0xffffffffu, row_slot, from),
+                           __shfl_sync(0xffffffffu, row_len, from), x0 - __shfl_sync(0xffffffffu, at, from));
+                break;
             }
-            at += w[j];
+            before += part.y;
         }
     }
-    __syncthreads();
-    Walk walk;
-    walk.begin(a, x0, x1, sh.start_row, sh.start_before);
     const long long limit = a.timeout_cycles;
+    // Query rows of the segments under way: 1, 2 or 4 of them in the 16-row buffer.
+    const int q_slots = NT > 1 ? 1 : (a.group > 4 ? 2 : 4), q_step = kUnitRows / q_slots * kQPitch;
 
     if (warp == 4) {
         // ---------------------------------------------------------------- loads
@@ -224,28 +244,29 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
         bool ok = true;
         while (ok && walk.next(a)) {
             const int head = walk.unit / a.chunks, chunk = walk.unit - head * a.chunks;
-            const int rows = min(kUnitRows, a.group - chunk * kUnitRows);
+            const int rows = min(8 * NT, a.group - chunk * 8 * NT);
             const int32_t* table = a.table + static_cast<long long>(walk.slot) * a.max_pages;
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.q_empty[seg & 1], ((seg >> 1) & 1) ^ 1, abort_flag, limit));
-            if (!ok) break;
-            const uint32_t row_bytes = a.head_dim * 2;
-            if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[seg & 1], rows * row_bytes);
-            __syncwarp();
-            if (lane < rows)
-                bulk_load(sq + (seg & 1) * kUnitRows * kQPitch + lane * kQPitch,
-                          a.q + static_cast<long long>(walk.i) * a.q_seq +
-                              static_cast<long long>(head * a.group + chunk * kUnitRows + lane) * a.q_head,
-                          row_bytes, &sh.q_full[seg & 1]);
-            ++seg;
             // lane p < pieces loads piece p of every tile; its page is looked up one tile ahead
             auto lookup = [&](int t) {
-                const long long tok = static_cast<long long>(t) * kTokens + lane * a.box;
+                const int tok = t * kTokens + lane * a.box;
                 return lane < pieces && tok < walk.len ? table[tok / a.page_size] : -1;
             };
             int page = lookup(walk.t0);
+            const int qs = seg & (q_slots - 1);
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.q_empty[qs], ((seg / q_slots) & 1) ^ 1, abort_flag, limit));
+            if (!ok) break;
+            const uint32_t row_bytes = a.head_dim * 2;
+            if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[qs], rows * row_bytes);
+            __syncwarp();
+            if (lane < rows)
+                bulk_load(sq + qs * q_step + lane * kQPitch,
+                          a.q + static_cast<long long>(walk.i) * a.q_seq +
+                              static_cast<long long>(head * a.group + chunk * 8 * NT + lane) * a.q_head,
+                          row_bytes, &sh.q_full[qs]);
+            ++seg;
             for (int t = walk.t0; t < walk.t1; ++t, ++it) {
-                const int s = it % kDecodeStages;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.empty[s], ((it / kDecodeStages) & 1) ^ 1, abort_flag, limit));
+                const int s = it % S;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.empty[s], ((it / S) & 1) ^ 1, abort_flag, limit));
                 if (!ok) break;
                 const int tok = t * kTokens + lane * a.box;
                 const bool mine = lane < pieces && tok < walk.len;
@@ -275,10 +296,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
             *abort_flag = 1;
         }
         // every issued load lands before the CTA may exit
-        for (uint32_t i = it > kDecodeStages ? it - kDecodeStages : 0; i < it; ++i)
-            mbar_wait_bounded(&sh.full[i % kDecodeStages], (i / kDecodeStages) & 1, nullptr, drain);
-        for (uint32_t i = seg > 2 ? seg - 2 : 0; i < seg; ++i)
-            mbar_wait_bounded(&sh.q_full[i & 1], (i >> 1) & 1, nullptr, drain);
+        for (uint32_t i = it > S ? it - S : 0; i < it; ++i)
+            mbar_wait_bounded(&sh.full[i % S], (i / S) & 1, nullptr, drain);
+        for (uint32_t i = seg > static_cast<uint32_t>(q_slots) ? seg - q_slots : 0; i < seg; ++i)
+            mbar_wait_bounded(&sh.q_full[i & (q_slots - 1)], (i / q_slots) & 1, nullptr, drain);
         return;
     }
 
@@ -297,222 +318,248 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
     uint32_t it = 0, seg = 0;
     while (walk.next(a)) {
         const int head = walk.unit / a.chunks, chunk = walk.unit - head * a.chunks;
-        const int rows = min(kUnitRows, a.group - chunk * kUnitRows);
-        // Q fragments
-        uint32_t qf[4 * DCH][4];
-        wait(&sh.q_full[seg & 1], (seg >> 1) & 1);
-        {
-            const uint32_t qa = smem_u32(sq + (seg & 1) * kUnitRows * kQPitch) + ((mat & 1) * 8 + mrow) * kQPitch + (mat >> 1) * 16;
+        const int rows = min(8 * NT, a.group - chunk * 8 * NT);
+        // Q^T as right operands
+        uint32_t qf[NT][4 * DCH][2];
+        const int qs = seg & (q_slots - 1);
+        wait(&sh.q_full[qs], (seg / q_slots) & 1);
 #pragma unroll
-            for (int k = 0; k < 4 * DCH; ++k) {
-                if (k < ksteps) ldmatrix_x4(qa + k * 32, qf[k]);
-                if (r0 >= rows) qf[k][0] = qf[k][2] = 0;
-                if (r0 + 8 >= rows) qf[k][1] = qf[k][3] = 0;
+        for (int h = 0; h < NT; ++h) {
+            // (rows past the unit's are whatever lies there, and are set to 0)
+            const uint32_t qa = smem_u32(sq) + qs * q_step + (8 * h + mrow) * kQPitch + mat * 16;
+#pragma unroll
+            for (int k = 0; k < 4 * DCH; k += 2) {
+                uint32_t b[4] = {0, 0, 0, 0};
+                if (k < ksteps) ldmatrix_x4(qa + k * 32, b);
+                const bool row = 8 * h + r0 < rows;
+                qf[h][k][0] = row ? b[0] : 0u;
+                qf[h][k][1] = row ? b[1] : 0u;
+                qf[h][k + 1][0] = row ? b[2] : 0u;
+                qf[h][k + 1][1] = row ? b[3] : 0u;
             }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.q_empty[seg & 1]);
+        if (lane == 0) mbar_arrive(&sh.q_empty[qs]);
         ++seg;
-        float o[DCH][2][4] = {};        // head_dim pairs of 8: pair warp + 4 c
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        float o[DCH][NT][4] = {};       // O^T: 16 dimensions by 8 rows each, dimensions 16 (warp + 4 d)
+        float m[NT][2], l[NT][2];       // of rows 8 h + cpair and the next
+#pragma unroll
+        for (int h = 0; h < NT; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[h][e] = -INFINITY;
+                l[h][e] = 0.f;
+            }
         for (int t = walk.t0; t < walk.t1; ++t, ++it) {
-            const int s = it % kDecodeStages;
+            const int s = it % S;
             const uint32_t kb = smem_u32(ring + s * Cfg::kStage), vb = kb + Cfg::kTensor;
-            wait(&sh.full[s], (it / kDecodeStages) & 1);
-            // scores of this warp's 16 keys
-            float c[2][4] = {};
+            wait(&sh.full[s], (it / S) & 1);
+            const int live = walk.len - t * kTokens;  // keys of the tile that exist
+            float c[NT][4] = {}, d[NT][4] = {};
             {
-                const int tok = 16 * warp + (mat >> 1) * 8 + mrow;
+                const int tok = 16 * warp + (mat & 1) * 8 + mrow;
                 const uint32_t ka = kb + tok * 128;
 #pragma unroll
                 for (int k = 0; k < 4 * DCH; ++k) {
                     if (k < ksteps) {
-                        uint32_t b[4];
-                        const int v = (2 * k + (mat & 1)) & 7;
-                        ldmatrix_x4(ka + (k >> 2) * (kTokens * 128) + ((v ^ (tok & 7)) << 4), b);
-                        mma_16816<BF16>(c[0], qf[k], b[0], b[1]);
-                        mma_16816<BF16>(c[1], qf[k], b[2], b[3]);
+                        uint32_t x[4];
+                        const int v = (2 * k + (mat >> 1)) & 7;
+                        ldmatrix_x4(ka + (k >> 2) * (kTokens * 128) + ((v ^ (tok & 7)) << 4), x);
+                        // (even and odd steps in sums of their own: half the chain)
+#pragma unroll
+                        for (int h = 0; h < NT; ++h) mma_16816<BF16>(k & 1 ? d[h] : c[h], x, qf[h][k][0], qf[h][k][1]);
                     }
                 }
             }
-            const int live = walk.len - t * kTokens;  // keys of the tile that exist
-            if (live < kTokens) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+            for (int h = 0; h < NT; ++h) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (16 * warp + 8 * j + cpair + (e & 1) >= live) c[j][e] = -INFINITY;
-            }
-            float t0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
-            float t1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
-            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
-            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
-            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
-            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-            if ((lane & 3) == 0) {
-                sh.top[warp][r0] = t0;
-                sh.top[warp][r0 + 8] = t1;
+                for (int e = 0; e < 4; ++e) {
+                    c[h][e] += d[h][e];
+                    if (16 * warp + r0 + (e & 2) * 4 >= live) c[h][e] = -INFINITY;
+                }
+                float top[2] = {fmaxf(c[h][0], c[h][2]), fmaxf(c[h][1], c[h][3])};
+#pragma unroll
+                for (int i = 4; i < 32; i *= 2) {
+                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], i));
+                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], i));
+                }
+                if (r0 == 0) *reinterpret_cast<float2*>(&sh.top[warp][8 * h + cpair]) = make_float2(top[0], top[1]);
             }
             consumer_sync();
-            t0 = fmaxf(fmaxf(sh.top[0][r0], sh.top[1][r0]), fmaxf(sh.top[2][r0], sh.top[3][r0])) * a.scale_log2;
-            t1 = fmaxf(fmaxf(sh.top[0][r0 + 8], sh.top[1][r0 + 8]), fmaxf(sh.top[2][r0 + 8], sh.top[3][r0 + 8])) * a.scale_log2;
-            const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-            const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-            const float f0 = exp2_fast(m0 - b0), f1 = exp2_fast(m1 - b1);
-            m0 = n0;
-            m1 = n1;
-            l0 *= f0;
-            l1 *= f1;
-            uint8_t* pw = sp + r0 * kPPitch + (16 * warp + cpair) * 2;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float u0 = exp2_fast(fmaf(c[j][0], a.scale_log2, -b0)), u1 = exp2_fast(fmaf(c[j][1], a.scale_log2, -b0));
-                const float w0 = exp2_fast(fmaf(c[j][2], a.scale_log2, -b1)), w1 = exp2_fast(fmaf(c[j][3], a.scale_log2, -b1));
-                l0 += u0 + u1;
-                l1 += w0 + w1;
-                *reinterpret_cast<uint32_t*>(pw + 16 * j) = pack2<BF16>(u0, u1);
-                *reinterpret_cast<uint32_t*>(pw + 8 * kPPitch + 16 * j) = pack2<BF16>(w0, w1);
+            for (int h = 0; h < NT; ++h) {
+                float2 w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float2*>(&sh.top[i][8 * h + cpair]);
+                const float top[2] = {fmaxf(fmaxf(w[0].x, w[1].x), fmaxf(w[2].x, w[3].x)) * a.scale_log2,
+                                      fmaxf(fmaxf(w[0].y, w[1].y), fmaxf(w[2].y, w[3].y)) * a.scale_log2};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mm = fmaxf(m[h][e], top[e]), b = mm == -INFINITY ? 0.f : mm;
+                    const float f = exp2_fast(m[h][e] - b);
+                    m[h][e] = mm;
+                    c[h][e] = exp2_fast(fmaf(c[h][e], a.scale_log2, -b));
+                    c[h][e + 2] = exp2_fast(fmaf(c[h][e + 2], a.scale_log2, -b));
+                    l[h][e] = l[h][e] * f + c[h][e] + c[h][e + 2];
+#pragma unroll
+                    for (int i = 0; i < DCH; ++i) {
+                        o[i][h][e] *= f;
+                        o[i][h][e + 2] *= f;
+                    }
+                }
+                // the weights by rows, 16 of this warp's keys
+                uint8_t* pw = sp + (8 * h + r0) * kPPitch + (16 * warp + cpair) * 2;
+                *reinterpret_cast<uint32_t*>(pw) = movmatrix_trans(pack2<BF16>(c[h][0], c[h][1]));
+                *reinterpret_cast<uint32_t*>(pw + 16) = movmatrix_trans(pack2<BF16>(c[h][2], c[h][3]));
             }
+            consumer_sync();
+            // O^T += V^T P^T over all 64 keys, this warp's part of head_dim
+            const uint32_t pa = smem_u32(sp) + mrow * kPPitch + mat * 16;
 #pragma unroll
-            for (int d = 0; d < DCH; ++d)
+            for (int k = 0; k < kTokens / 16; k += 2) {
+                uint32_t p[NT][4];
+#pragma unroll
+                for (int h = 0; h < NT; ++h) ldmatrix_x4(pa + 8 * h * kPPitch + k * 32, p[h]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    o[d][j][0] *= f0;
-                    o[d][j][1] *= f0;
-                    o[d][j][2] *= f1;
-                    o[d][j][3] *= f1;
-                }
-            consumer_sync();
-            // O += P V over all 64 keys, this warp's part of head_dim
-            const uint32_t pa = smem_u32(sp) + ((mat & 1) * 8 + mrow) * kPPitch + (mat >> 1) * 16;
+                    const int tok = 16 * (k + j) + (mat >> 1) * 8 + mrow;
+                    // keys past the end have weight 0, but what lies in their place may be NaN
+                    const int left = live - 16 * (k + j) - cpair;
+                    const uint32_t lo = left >= 2 ? 0xFFFFFFFFu : (left == 1 ? 0x0000FFFFu : 0u);
+                    const uint32_t hi = left >= 10 ? 0xFFFFFFFFu : (left == 9 ? 0x0000FFFFu : 0u);
 #pragma unroll
-            for (int k = 0; k < kTokens / 16; ++k) {
-                uint32_t p[4];
-                ldmatrix_x4(pa + k * 32, p);
-                const int tok = 16 * k + (mat & 1) * 8 + mrow;
-                // keys past the end have weight 0, but what lies in their place may be NaN
-                const int left = live - 16 * k - cpair;
-                const uint32_t lo = left >= 2 ? 0xFFFFFFFFu : (left == 1 ? 0x0000FFFFu : 0u);
-                const uint32_t hi = left >= 10 ? 0xFFFFFFFFu : (left == 9 ? 0x0000FFFFu : 0u);
+                    for (int i = 0; i < DCH; ++i) {
+                        const int part = warp + 4 * i;
+                        if (part < ksteps) {
+                            uint32_t x[4];
+                            const int v = (2 * part + (mat & 1)) & 7;
+                            ldmatrix_x4_trans(vb + (part >> 2) * (kTokens * 128) + tok * 128 + ((v ^ (tok & 7)) << 4), x);
+                            x[0] &= lo;
+                            x[1] &= lo;
+                            x[2] &= hi;
+                            x[3] &= hi;
 #pragma unroll
-                for (int d = 0; d < DCH; ++d) {
-                    const int pair = warp + 4 * d;
-                    if (pair < ksteps) {
-                        uint32_t b[4];
-                        const int v = (2 * pair + (mat >> 1)) & 7;
-                        ldmatrix_x4_trans(vb + (pair >> 2) * (kTokens * 128) + tok * 128 + ((v ^ (tok & 7)) << 4), b);
-                        mma_16816<BF16>(o[d][0], p, b[0] & lo, b[1] & hi);
-                        mma_16816<BF16>(o[d][1], p, b[2] & lo, b[3] & hi);
+                            for (int h = 0; h < NT; ++h) mma_16816<BF16>(o[i][h], x, p[h][2 * j], p[h][2 * j + 1]);
+                        }
                     }
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.empty[s]);
         }
-        // the sum of weights over the quad and the four warps
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        if ((lane & 3) == 0) {
-            sh.sum[warp][r0] = l0;
-            sh.sum[warp][r0 + 8] = l1;
-        }
+        // ---------------------------------------------------------------- the unit's end
+#pragma unroll
+        for (int h = 0; h < NT; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int i = 4; i < 32; i *= 2) l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], i);
+                if (r0 == 0) sh.sum[warp][8 * h + cpair + e] = l[h][e];
+            }
         consumer_sync();
-        l0 = (sh.sum[0][r0] + sh.sum[1][r0]) + (sh.sum[2][r0] + sh.sum[3][r0]);
-        l1 = (sh.sum[0][r0 + 8] + sh.sum[1][r0 + 8]) + (sh.sum[2][r0 + 8] + sh.sum[3][r0 + 8]);
-        const int qh = head * a.group + chunk * kUnitRows;  // the unit's first query head
+        const int qh = head * a.group + chunk * 8 * NT;  // the unit's first query head
         uint16_t* out = a.out + static_cast<long long>(walk.i) * a.o_seq + static_cast<long long>(qh) * a.o_head;
         float* lse = a.lse ? a.lse + static_cast<long long>(walk.i) * a.q_heads + qh : nullptr;
-        const bool any = walk.len > 0;
-        if (walk.t0 == 0 && walk.t1 == walk.nt) {
-            const float i0 = any ? 1.f / l0 : 0.f, i1 = any ? 1.f / l1 : 0.f;
-#pragma unroll
-            for (int d = 0; d < DCH; ++d) {
-                const int pair = warp + 4 * d;
-                if (pair >= ksteps) continue;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int col = 16 * pair + 8 * j + cpair;
-                    if (r0 < rows)
-                        *reinterpret_cast<uint32_t*>(out + r0 * a.o_head + col) = any ? pack2<BF16>(o[d][j][0] * i0, o[d][j][1] * i0) : 0u;
-                    if (r0 + 8 < rows)
-                        *reinterpret_cast<uint32_t*>(out + (r0 + 8) * a.o_head + col) = any ? pack2<BF16>(o[d][j][2] * i1, o[d][j][3] * i1) : 0u;
-                }
-            }
-            if (lse != nullptr && warp == 0 && (lane & 3) == 0) {
-                if (r0 < rows) lse[r0] = any ? ((m0 == -INFINITY ? 0.f : m0) + log2f(l0)) * kLn2 : -INFINITY;
-                if (r0 + 8 < rows) lse[r0 + 8] = any ? ((m1 == -INFINITY ? 0.f : m1) + log2f(l1)) * kLn2 : -INFINITY;
-            }
-            continue;
-        }
-        // A part of a unit. Parts that begin a unit lie in a CTA's second place, others in its first.
-        auto cta_of = [&](long long x) { return ((x + 1) * ctas - 1) / total; };
-        const long long c0 = cta_of(walk.unit_start), c1 = cta_of(walk.unit_start + walk.nt - 1);
+        const bool whole = walk.t0 == 0 && walk.t1 == walk.nt;
+        // Parts that begin a unit lie in a CTA's second place, others in its first.
         const long long place = 2ll * blockIdx.x + (walk.t0 == 0 ? 1 : 0);
         float* po = a.part_o + place * kUnitRows * a.head_dim;
 #pragma unroll
-        for (int d = 0; d < DCH; ++d) {
-            const int pair = warp + 4 * d;
-            if (pair >= ksteps) continue;
+        for (int h = 0; h < NT; ++h) {
+            float inv[2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int col = 16 * pair + 8 * j + cpair;
-                if (r0 < rows) *reinterpret_cast<float2*>(po + r0 * a.head_dim + col) = make_float2(o[d][j][0], o[d][j][1]);
-                if (r0 + 8 < rows) *reinterpret_cast<float2*>(po + (r0 + 8) * a.head_dim + col) = make_float2(o[d][j][2], o[d][j][3]);
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * h + cpair + e;
+                const float sum = (sh.sum[0][row] + sh.sum[1][row]) + (sh.sum[2][row] + sh.sum[3][row]);
+                inv[e] = walk.len > 0 ? __fdividef(1.f, sum) : 0.f;
+                if (warp == 0 && r0 == 0 && row < rows) {
+                    if (!whole) a.part_ml[place * kUnitRows + row] = make_float2(m[h][e], sum);
+                    else if (lse != nullptr) lse[row] = m[h][e] == -INFINITY ? -INFINITY : (m[h][e] + __log2f(sum)) * kLn2;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < DCH; ++i) {
+                const int dim = 16 * (warp + 4 * i);
+                if (dim >= a.head_dim) continue;
+                if (whole) {
+                    // by rows: two dimensions a lane
+                    const uint32_t x = movmatrix_trans(pack2<BF16>(o[i][h][0] * inv[0], o[i][h][1] * inv[1]));
+                    const uint32_t y = movmatrix_trans(pack2<BF16>(o[i][h][2] * inv[0], o[i][h][3] * inv[1]));
+                    if (8 * h + r0 < rows) {
+                        uint16_t* dst = out + (8 * h + r0) * a.o_head + dim + cpair;
+                        *reinterpret_cast<uint32_t*>(dst) = x;
+                        *reinterpret_cast<uint32_t*>(dst + 8) = y;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = 8 * h + cpair + (e & 1);
+                        if (row < rows) po[row * a.head_dim + dim + r0 + (e & 2) * 4] = o[i][h][e];
+                    }
+                }
             }
         }
-        if (warp == 0 && (lane & 3) == 0) {
-            a.part_ml[place * kUnitRows + r0] = make_float2(m0, l0);
-            a.part_ml[place * kUnitRows + r0 + 8] = make_float2(m1, l1);
-        }
-        __threadfence();
-        consumer_sync();
+        if (whole) continue;
+        consumer_sync();  // the part has been written
+        const long long c0 = cta_of(walk.unit_start), c1 = cta_of(walk.unit_start + walk.nt - 1);
+        const int parts = static_cast<int>(c1 - c0) + 1;
         if (threadIdx.x == 0) {
-            const uint32_t parts = static_cast<uint32_t>(c1 - c0 + 1);
-            const bool last = atomicAdd(a.arrived + c0, 1u) == parts - 1;
+            // releases what the barrier above has shown this thread, and acquires the other parts
+            uint32_t old;
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(a.arrived + c0) : "memory");
+            const bool last = old == static_cast<uint32_t>(parts - 1);
             if (last) a.arrived[c0] = 0;  // nobody else of this call comes here any more
             sh.last = last;
-            __threadfence();
         }
         consumer_sync();
         if (sh.last) {
-            // the parts in the order of the keys: c0's second place, the others' first
+            // the parts in the order of the keys: c0's second place, the others' first; eight of them loaded at a time
+            constexpr int kBatch = 8;
             const int vecs = a.head_dim / 4;
+            const float2* ml0 = a.part_ml + 2 * c0 * kUnitRows;
+            const float* o0 = a.part_o + 2 * c0 * kUnitRows * a.head_dim;
             for (int e = threadIdx.x; e < rows * vecs; e += kConsumers) {
                 const int row = e / vecs, v = e - row * vecs;
-                float m = -INFINITY, l = 0.f;
+                float mm = -INFINITY, ll = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (long long c = c0; c <= c1; c += 4) {
-                    float2 ml[4];
-                    float4 x[4];
+#pragma unroll 1
+                for (int c = 0; c < parts; c += kBatch) {
+                    float2 ml[kBatch];
+                    float4 x[kBatch];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (c + j > c1) continue;
-                        const long long from = 2 * (c + j) + (c + j == c0 ? 1 : 0);
-                        ml[j] = __ldcg(a.part_ml + from * kUnitRows + row);
-                        x[j] = __ldcg(reinterpret_cast<const float4*>(a.part_o + (from * kUnitRows + row) * a.head_dim) + v);
+                    for (int j = 0; j < kBatch; ++j) {
+                        ml[j] = make_float2(-INFINITY, 0.f);
+                        x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (c + j < parts) {
+                            const int at = (2 * (c + j) + (c + j == 0 ? 1 : 0)) * kUnitRows + row;
+                            ml[j] = __ldcg(ml0 + at);
+                            x[j] = __ldcg(reinterpret_cast<const float4*>(o0 + static_cast<long long>(at) * a.head_dim) + v);
+                        }
                     }
+                    float top = mm;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (c + j > c1) continue;
-                        const float mm = fmaxf(m, ml[j].x), b = mm == -INFINITY ? 0.f : mm;
-                        const float f = exp2_fast(m - b), g = exp2_fast(ml[j].x - b);
-                        m = mm;
-                        l = l * f + ml[j].y * g;
-                        acc.x = acc.x * f + x[j].x * g;
-                        acc.y = acc.y * f + x[j].y * g;
-                        acc.z = acc.z * f + x[j].z * g;
-                        acc.w = acc.w * f + x[j].w * g;
+                    for (int j = 0; j < kBatch; ++j) top = fmaxf(top, ml[j].x);
+                    const float b = top == -INFINITY ? 0.f : top, f = exp2_fast(mm - b);
+                    mm = top;
+                    ll *= f;
+                    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const float g = exp2_fast(ml[j].x - b);
+                        ll = fmaf(ml[j].y, g, ll);
+                        acc.x = fmaf(x[j].x, g, acc.x);
+                        acc.y = fmaf(x[j].y, g, acc.y);
+                        acc.z = fmaf(x[j].z, g, acc.z);
+                        acc.w = fmaf(x[j].w, g, acc.w);
                     }
                 }
-                const float inv = 1.f / l;  // (a unit in parts has tokens)
+                const float inv = __fdividef(1.f, ll);  // (a unit in parts has tokens)
                 *reinterpret_cast<uint2*>(out + row * a.o_head + 4 * v) =
                     make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
-                if (lse != nullptr && v == 0) lse[row] = ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2;
+                if (lse != nullptr && v == 0) lse[row] = mm == -INFINITY ? -INFINITY : (mm + __log2f(ll)) * kLn2;
             }
         }
-        consumer_sync();  // sh.last and sh.sum are free again
     }
 }
 
@@ -555,9 +602,9 @@ void decode_destroy(tb_cache* c) {
     if (c->arrived) cudaFree(c->arrived);
 }
 
-template <bool BF16, int DCH>
+template <bool BF16, int DCH, int NT>
 static tb_status launch_decode(tb_cache* c, int layer, const DecodeArgs& a, cudaStream_t st) {
-    auto* kernel = decode_kernel<BF16, DCH>;
+    auto* kernel = decode_kernel<BF16, DCH, NT>;
     static bool ready = false;  // the attribute is per function and process-wide
     if (!ready) {
         TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<DCH>::kSmem));
@@ -576,6 +623,14 @@ static tb_status launch_decode(tb_cache* c, int layer, const DecodeArgs& a, cuda
     TB_CUDA(cudaLaunchKernelEx(&cfg, kernel, c->k_map[layer], c->v_map[layer], a));
     c->ctx->launches++;
     return TB_OK;
+}
+
+template <bool BF16>
+static tb_status launch_decode(tb_cache* c, int layer, const DecodeArgs& a, cudaStream_t st) {
+    // groups above 8 would read every key once more for each 8 query heads: 16 of them share a unit there
+    const bool two = a.group > 8;
+    if (a.head_dim > 64) return two ? launch_decode<BF16, 2, 2>(c, layer, a, st) : launch_decode<BF16, 2, 1>(c, layer, a, st);
+    return two ? launch_decode<BF16, 1, 2>(c, layer, a, st) : launch_decode<BF16, 1, 1>(c, layer, a, st);
 }
 
 }  // namespace tb
@@ -615,7 +670,8 @@ TB_API tb_status tb_cache_attend(tb_cache* c, int32_t layer, const int32_t* slot
     a.q_heads = q_heads;
     a.kv_heads = d.kv_heads;
     a.group = group;
-    a.chunks = (group + kUnitRows - 1) / kUnitRows;
+    const int unit = group > 8 ? 16 : 8;
+    a.chunks = (group + unit - 1) / unit;
     a.head_dim = d.head_dim;
     a.page_size = d.page_size;
     a.num_pages = d.num_pages;
@@ -629,10 +685,7 @@ TB_API tb_status tb_cache_attend(tb_cache* c, int32_t layer, const int32_t* slot
     a.err = c->ctx->dev_err;
     a.timeout_cycles = c->ctx->timeout_cycles;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool wide = d.head_dim > 64;
-    if (d.dtype == TB_DT_BF16)
-        return wide ? launch_decode<true, 2>(c, layer, a, st) : launch_decode<true, 1>(c, layer, a, st);
-    return wide ? launch_decode<false, 2>(c, layer, a, st) : launch_decode<false, 1>(c, layer, a, st);
+    return d.dtype == TB_DT_BF16 ? launch_decode<true>(c, layer, a, st) : launch_decode<false>(c, layer, a, st);
 }
 
 }  // extern "C"
