@@ -1,10 +1,12 @@
-"""Build libtosa_b200.so in-tree for sm_100a (nvcc cross-compiles without a GPU).
+"""Build libtosa_b200.so and its torch binding in-tree for sm_100a (nvcc cross-compiles without a GPU).
 
 Usage: python -m tosa_b200.build [--force]
 
 Each translation unit under csrc/ is compiled in parallel into _build/ and the
 objects are linked into tosa_b200/libtosa_b200.so (CUDA runtime linked
 statically; driver entry points are resolved at run time).
+csrc/torch_binding.cpp is compiled with the host compiler against the
+installed torch into tosa_b200/_torch_binding.so, which loads that library.
 """
 
 from __future__ import annotations
@@ -18,6 +20,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "libtosa_b200.so")
+BINDING_SRC = os.path.join(CSRC, "torch_binding.cpp")
+BINDING = os.path.join(HERE, "_torch_binding.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -29,14 +33,58 @@ def _sources():
 
 
 def _newest_input():
-    files = glob.glob(os.path.join(CSRC, "*")) + glob.glob(os.path.join(HERE, "..", "include", "*.h"))
+    files = [f for f in glob.glob(os.path.join(CSRC, "*")) if f != BINDING_SRC] + glob.glob(os.path.join(HERE, "..", "include", "*.h"))
     return max(os.path.getmtime(f) for f in files)
 
 
+def _start_binding(force, verbose):
+    """Starts compiling the torch binding when it is out of date; returns the process or None."""
+    inputs = [BINDING_SRC] + glob.glob(os.path.join(HERE, "..", "include", "*.h"))
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(f) for f in inputs):
+        return None
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    obj = os.path.join(BUILD, "torch_binding.cpp.o")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-c", "-o", obj, BINDING_SRC,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", os.path.join(root, "include"),
+           "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"), "-isystem",
+           os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"]]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    return subprocess.Popen(cmd), obj, os.path.join(root, "lib")
+
+
+def _link_binding(started, verbose):
+    process, obj, libs = started
+    if process.wait() != 0:
+        raise RuntimeError(f"the host compiler failed for {BINDING_SRC}")
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", BINDING + ".tmp", obj, "-L" + HERE, "-l:libtosa_b200.so", "-L" + libs,
+           "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    os.replace(BINDING + ".tmp", BINDING)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    os.makedirs(BUILD, exist_ok=True)
+    binding = _start_binding(force, verbose)
+    try:
+        out = _build_library(force, verbose)
+    finally:
+        if binding is not None:
+            binding[0].wait()
+    if binding is not None:
+        _link_binding(binding, verbose)
+    return out
+
+
+def _build_library(force: bool, verbose: bool) -> str:
     if not force and os.path.exists(OUT) and os.path.getmtime(OUT) >= _newest_input():
         return OUT
-    os.makedirs(BUILD, exist_ok=True)
     newest_header = max(os.path.getmtime(f) for f in glob.glob(os.path.join(CSRC, "*.cuh")) +
                         glob.glob(os.path.join(CSRC, "*.hpp")) + glob.glob(os.path.join(HERE, "..", "include", "*.h")))
     procs, objs = [], []
