@@ -6,8 +6,11 @@
 // bookkeeping is one block of 1024 threads: prefix sums over the slots' needs and
 // over the free pages, no atomics whose order could show in the result. It checks
 // everything before it changes anything, so a refused call leaves the state as it
-// was. Moving page contents is a second, grid-wide kernel that reads the list the
-// first one left; it is bound by memory bandwidth.
+// was. Such a block's time is its chain of dependent accesses, some 0.7 us each: values that
+// only the end of a call changes are read through L1, eight lanes take a slot's pages so that 128 slots
+// are looked at together, and checks share a barrier (fork of 64 children: 17 -> 10 us). Moving
+// page contents is a second, grid-wide kernel that reads the list the first one left; it is bound by
+// memory bandwidth.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -117,35 +120,23 @@ __device__ void clear_marks(const CacheView& c, const int32_t* slots, int n) {
     }
 }
 
-// Whether every page of the slots (marked, so of valid length) is a page of the pool. A warp a slot.
-__device__ bool pages_ok(const CacheView& c, const int32_t* slots, int n) {
-    bool bad = false;
-    for (int i = threadIdx.x >> 5; i < n; i += kBook / 32) {
-        const int s = slots[i];
-        const int np = pages_for(__ldcg(c.lengths + s), c.page_size);
-        for (int j = threadIdx.x & 31; j < np; j += 32) {
-            const int p = __ldcg(c.table + static_cast<long long>(s) * c.max_pages + j);
-            if (p < 0 || p >= c.num_pages) bad = true;
-        }
-    }
-    return !__syncthreads_or(bad);
-}
-
-// refs += add for the first pages of each slot: all of them, or only those filled to the end.
-__device__ void add_refs(const CacheView& c, const int32_t* slots, int n, bool full_only, int add) {
-    for (int i = threadIdx.x >> 5; i < n; i += kBook / 32) {
-        const int s = slots[i];
-        const int len = __ldcg(c.lengths + s);
+// Eight lanes a slot: calls f(page) for the first pages of the slots i0, i0 + 128, ...: all of them, or only
+// those filled to the end. lengths and table change only at a call's end, so they may come from L1.
+template <class F>
+__device__ __forceinline__ void for_pages(const CacheView& c, const int32_t* slots, int n, bool full_only, F f) {
+    for (int i = threadIdx.x >> 3; i < n; i += kBook / 8) {
+        const int s = slots[i], len = c.lengths[s];
         const int np = full_only ? len / c.page_size : pages_for(len, c.page_size);
-        for (int j = threadIdx.x & 31; j < np; j += 32)
-            atomicAdd(c.refs + __ldcg(c.table + static_cast<long long>(s) * c.max_pages + j), add);
+        const int32_t* row = c.table + static_cast<long long>(s) * c.max_pages;
+#pragma unroll 4
+        for (int j = threadIdx.x & 7; j < np; j += 8) f(row[j]);
     }
-    __syncthreads();
 }
 
 __global__ void __launch_bounds__(kBook) cache_reserve_kernel(CacheView c, const int32_t* slots, const int32_t* counts,
                                                               int n) {
     __shared__ int s[33];
+    if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
     bool bad = !mark_slots(c, slots, n);
     if (!bad) {
@@ -198,16 +189,21 @@ __global__ void __launch_bounds__(kBook) cache_reserve_kernel(CacheView c, const
 }
 
 __global__ void __launch_bounds__(kBook) cache_free_kernel(CacheView c, const int32_t* slots, int n) {
+    if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
-    const bool ok = mark_slots(c, slots, n) && pages_ok(c, slots, n);
-    if (ok) {
-        add_refs(c, slots, n, false, -1);
-        for (int i = threadIdx.x >> 5; i < n; i += kBook / 32) {
-            const int slot = slots[i];
-            const int np = pages_for(__ldcg(c.lengths + slot), c.page_size);
-            for (int j = threadIdx.x & 31; j < np; j += 32) c.table[static_cast<long long>(slot) * c.max_pages + j] = -1;
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) c.lengths[slot] = 0;
+    bool bad = !mark_slots(c, slots, n);
+    if (!bad) {
+        for_pages(c, slots, n, false, [&](int p) { bad |= p < 0 || p >= c.num_pages; });
+        bad = __syncthreads_or(bad);
+    }
+    if (!bad) {
+        for_pages(c, slots, n, false, [&](int p) { atomicSub(c.refs + p, 1); });
+        __syncthreads();  // every row has been read
+        for (int i = threadIdx.x >> 3; i < n; i += kBook / 8) {
+            const int slot = slots[i], np = pages_for(c.lengths[slot], c.page_size);
+            for (int j = threadIdx.x & 7; j < np; j += 8) c.table[static_cast<long long>(slot) * c.max_pages + j] = -1;
+            __syncwarp(0xFFu << (threadIdx.x & 24));
+            if ((threadIdx.x & 7) == 0) c.lengths[slot] = 0;
         }
     } else if (threadIdx.x == 0) {
         atomicOr(c.err, DEV_ERR_INDEX);
@@ -218,6 +214,7 @@ __global__ void __launch_bounds__(kBook) cache_free_kernel(CacheView c, const in
 __global__ void __launch_bounds__(kBook) cache_fork_kernel(CacheView c, const int32_t* parents, const int32_t* children,
                                                            int n) {
     __shared__ int s[33];
+    if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
     bool bad = !mark_slots(c, children, n);
     for (int i = threadIdx.x; i < n; i += kBook) {
@@ -225,45 +222,53 @@ __global__ void __launch_bounds__(kBook) cache_fork_kernel(CacheView c, const in
         if (p < 0 || p >= c.max_seqs || __ldcg(c.marks + p) != 0) {
             bad = true;
         } else {
-            const int len = __ldcg(c.lengths + p);
+            const int len = c.lengths[p];
             if (len < 0 || static_cast<long long>(len) > static_cast<long long>(c.max_pages) * c.page_size) bad = true;
         }
     }
     bad = __syncthreads_or(bad);
-    if (!bad) bad = !pages_ok(c, children, n) || !pages_ok(c, parents, n);
+    if (!bad) {
+        auto look = [&](int p) { bad |= p < 0 || p >= c.num_pages; };
+        for_pages(c, children, n, false, look);
+        for_pages(c, parents, n, false, look);
+        bad = __syncthreads_or(bad);
+    }
     uint32_t err = bad ? DEV_ERR_INDEX : 0u;
     if (!bad) {
-        add_refs(c, children, n, false, -1);  // what the children held goes back
-        add_refs(c, parents, n, true, 1);     // full pages are shared
-        int need = 0;                         // a page for each last page that is not full
+        // what the children held goes back, full pages are shared
+        for_pages(c, children, n, false, [&](int p) { atomicSub(c.refs + p, 1); });
+        for_pages(c, parents, n, true, [&](int p) { atomicAdd(c.refs + p, 1); });
+        int need = 0;  // a page for each last page that is not full
         for (int i0 = 0; i0 < n; i0 += kBook) {
             const int i = i0 + threadIdx.x;
-            const int w = i < n && __ldcg(c.lengths + parents[i]) % c.page_size != 0;
+            const int w = i < n && c.lengths[parents[i]] % c.page_size != 0;
             int total;
             const int at = block_scan(w, s, total);
             if (i < n) c.offsets[i] = need + at;
             need += total;
         }
+        __syncthreads();
         if (!find_free(c, need, s)) {
             err = DEV_ERR_PAGES;
-            add_refs(c, parents, n, true, -1);
-            add_refs(c, children, n, false, 1);
+            for_pages(c, parents, n, true, [&](int p) { atomicSub(c.refs + p, 1); });
+            for_pages(c, children, n, false, [&](int p) { atomicAdd(c.refs + p, 1); });
         } else {
-            for (int i = threadIdx.x >> 5; i < n; i += kBook / 32) {
-                const int lane = threadIdx.x & 31, child = children[i];
-                const int len = __ldcg(c.lengths + parents[i]);
+            for (int i = threadIdx.x >> 3; i < n; i += kBook / 8) {
+                const int lane = threadIdx.x & 7, child = children[i];
+                const int len = c.lengths[parents[i]];
                 const int32_t* from = c.table + static_cast<long long>(parents[i]) * c.max_pages;
                 int32_t* to = c.table + static_cast<long long>(child) * c.max_pages;
                 const int full = len / c.page_size, rows = len % c.page_size;
-                const int had = pages_for(__ldcg(c.lengths + child), c.page_size);
-                for (int j = lane; j < max(full, had); j += 32) to[j] = j < full ? __ldcg(from + j) : -1;
-                __syncwarp();
+                const int had = pages_for(c.lengths[child], c.page_size);
+#pragma unroll 4
+                for (int j = lane; j < max(full, had); j += 8) to[j] = j < full ? from[j] : -1;
+                __syncwarp(0xFFu << (threadIdx.x & 24));
                 if (lane == 0) {
                     if (rows != 0) {
                         const int at = __ldcg(c.offsets + i), p = __ldcg(c.taken + at);
                         to[full] = p;
                         c.refs[p] = 1;
-                        c.job_src[at] = __ldcg(from + full);
+                        c.job_src[at] = from[full];
                         c.job_dst[at] = p;
                         c.job_rows[at] = rows;
                     }
@@ -284,29 +289,33 @@ __global__ void __launch_bounds__(kBook) cache_fork_kernel(CacheView c, const in
 // above that number and the k-th free page below it.
 __global__ void __launch_bounds__(kBook) cache_compact_kernel(CacheView c, int32_t* refs_out) {
     __shared__ int s[33];
+    if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
-    int live = 0;
-    for (int p0 = 0; p0 < c.num_pages; p0 += 4 * kBook) {
-        const int p = p0 + 4 * static_cast<int>(threadIdx.x);
-        int n = 0;
+    constexpr int kStep = 4 * kBook;
+    int live = 0, r[4];
+    auto load = [&](int p) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) n += p + j < c.num_pages && __ldcg(c.refs + p + j) > 0;
+        for (int j = 0; j < 4; ++j) r[j] = p + j < c.num_pages ? __ldcg(c.refs + p + j) : 0;
+    };
+    for (int p0 = 0; p0 < c.num_pages; p0 += kStep) {
+        load(p0 + 4 * static_cast<int>(threadIdx.x));
         int total;
-        block_scan(n, s, total);
+        block_scan((r[0] > 0) + (r[1] > 0) + (r[2] > 0) + (r[3] > 0), s, total);
         live += total;
     }
     int moves = 0, holes = 0;
-    for (int p0 = 0; p0 < c.num_pages; p0 += 4 * kBook) {
+    for (int p0 = 0; p0 < c.num_pages; p0 += kStep) {
         const int p = p0 + 4 * static_cast<int>(threadIdx.x);
-        int r[4], n = 0, h = 0;
+        if (c.num_pages > kStep) load(p);  // (otherwise they are still there)
+        int n = 0;  // pages that move in the low half, holes in the high one: at most 4096 of each a step
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            r[j] = p + j < c.num_pages ? __ldcg(c.refs + p + j) : 0;
             n += p + j >= live && r[j] > 0;
-            h += p + j < live && r[j] <= 0;
+            n += (p + j < live && r[j] <= 0) << 16;
         }
-        int tn, th;
-        int an = moves + block_scan(n, s, tn), ah = holes + block_scan(h, s, th);
+        int total;
+        const int at = block_scan(n, s, total);
+        int an = moves + (at & 0xFFFF), ah = holes + (at >> 16);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (p + j >= live && r[j] > 0) {
@@ -320,8 +329,8 @@ __global__ void __launch_bounds__(kBook) cache_compact_kernel(CacheView c, int32
                 refs_out[p + j] = r[j];
             }
         }
-        moves += tn;
-        holes += th;
+        moves += total & 0xFFFF;
+        holes += total >> 16;
     }
     __syncthreads();
     for (int k = threadIdx.x; k < moves; k += kBook) {
@@ -354,6 +363,7 @@ struct CopyArgs {
 // A warp moves one head of one page (page_size * head_dim contiguous elements, 4 KB at 16 tokens of
 // 128), eight 16-byte vectors a lane in flight: bound by memory bandwidth.
 __global__ void __launch_bounds__(256) cache_copy_kernel(CopyArgs a) {
+    if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     const long long warps = static_cast<long long>(gridDim.x) * 8;
@@ -407,9 +417,12 @@ struct WriteArgs {
     uint32_t* err;
 };
 
-// A warp writes the key or the value of one token: heads * head_dim elements, 16-byte vectors. The
-// token's slot is found by a 32-way search of the offsets (two steps for up to 1024 slots).
+// A warp writes the key or the value of one token: heads * head_dim elements, eight 16-byte vectors a lane in
+// flight. The token's slot is found by a 32-way search of the offsets (two steps for up to 1024 slots).
+// VECS: vectors of a head (head_dim / 8), 0: any number.
+template <int VECS>
 __global__ void __launch_bounds__(128) cache_write_kernel(WriteArgs a) {
+    if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     const long long w = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
@@ -428,12 +441,12 @@ __global__ void __launch_bounds__(128) cache_write_kernel(WriteArgs a) {
     const int first = a.offsets[lo], end = a.offsets[lo + 1];
     const int slot = a.slots[lo];
     bool bad = t < first || t >= end || slot < 0 || slot >= a.max_seqs;
-    long long pos = -1;
-    int page = -1;
+    int pos = -1, page = -1;
     if (!bad) {
-        pos = static_cast<long long>(a.lengths[slot]) - (end - t);
-        bad = pos < 0 || pos >= static_cast<long long>(a.max_pages) * a.page_size;
+        const long long at = static_cast<long long>(a.lengths[slot]) - (end - t);
+        bad = at < 0 || at >= static_cast<long long>(a.max_pages) * a.page_size;
         if (!bad) {
+            pos = static_cast<int>(at);
             page = a.table[static_cast<long long>(slot) * a.max_pages + pos / a.page_size];
             bad = page < 0 || page >= a.num_pages;
         }
@@ -442,17 +455,25 @@ __global__ void __launch_bounds__(128) cache_write_kernel(WriteArgs a) {
         if (lane == 0) atomicOr(a.err, DEV_ERR_INDEX);
         return;
     }
+    const int row_vecs = VECS ? VECS : a.row_vecs;
     const bool is_v = w & 1;
     const uint4* from = is_v ? a.v + t * a.v_token : a.k + t * a.k_token;
     const long long hs = is_v ? a.v_head : a.k_head;
-    const long long page_vecs = static_cast<long long>(a.page_size) * a.row_vecs;
-    uint4* to = (is_v ? a.v_layer : a.k_layer) + static_cast<long long>(page) * a.heads * page_vecs +
-                (pos % a.page_size) * a.row_vecs;
-    const int vecs = a.heads * a.row_vecs;
-#pragma unroll 4
-    for (int i = lane; i < vecs; i += 32) {
-        const int h = i / a.row_vecs, x = i - h * a.row_vecs;
-        to[h * page_vecs + x] = from[h * hs + x];
+    const int page_vecs = a.page_size * row_vecs;  // (a page of all heads is below 2^30 rows)
+    uint4* to = (is_v ? a.v_layer : a.k_layer) + static_cast<long long>(page) * a.heads * page_vecs + (pos % a.page_size) * row_vecs;
+    const int vecs = a.heads * row_vecs;
+    for (int i0 = lane; i0 < vecs; i0 += 256) {
+        uint4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + 32 * j, h = i / row_vecs;
+            if (i < vecs) x[j] = __ldcs(from + h * hs + (i - h * row_vecs));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + 32 * j, h = i / row_vecs;
+            if (i < vecs) to[static_cast<long long>(h) * page_vecs + (i - h * row_vecs)] = x[j];
+        }
     }
 }
 
@@ -545,14 +566,17 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
     c->ctx = ctx;
     c->d = *d;
     c->b = *b;
+    // one allocation: the attention's workspace (16-byte pieces first), then the words that begin as zero
     const size_t words = 2 * static_cast<size_t>(d->max_seqs) + 5 * static_cast<size_t>(d->num_pages) + 4;
-    cudaError_t e = cudaMalloc(&c->blob, words * sizeof(int32_t));
-    if (e == cudaSuccess) e = cudaMemset(c->blob, 0, words * sizeof(int32_t));
+    const size_t parts = decode_bytes(c);
+    cudaError_t e = cudaMalloc(&c->blob, parts + words * sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->blob, 0, parts + words * sizeof(int32_t), nullptr);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // other streams may be the first to use it
     if (e != cudaSuccess) {
         tb_cache_destroy(c);
         return fail(TB_ERR_CUDA, "cache workspace: %s", cudaGetErrorString(e));
     }
-    int32_t* w = static_cast<int32_t*>(c->blob);
+    int32_t* w = reinterpret_cast<int32_t*>(static_cast<char*>(c->blob) + parts);
     c->jobs = w;
     c->marks = w + 4;
     c->offsets = c->marks + d->max_seqs;
@@ -573,7 +597,6 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
 TB_API void tb_cache_destroy(tb_cache* c) {
     if (!c) return;
     if (c->blob) cudaFree(c->blob);
-    decode_destroy(c);
     delete c;
 }
 
@@ -665,8 +688,9 @@ TB_API tb_status tb_cache_write(tb_cache* c, int32_t layer, const int32_t* slots
     a.max_pages = c->d.max_pages;
     a.total = total;
     a.err = c->ctx->dev_err;
-    return launch(c->ctx, cache_write_kernel, static_cast<int>((2 * total + 3) / 4), 128,
-                  static_cast<cudaStream_t>(stream), a);
+    // head_dim 128 and 64: the division by a head's vectors is a shift
+    auto* kernel = a.row_vecs == 16 ? cache_write_kernel<16> : (a.row_vecs == 8 ? cache_write_kernel<8> : cache_write_kernel<0>);
+    return launch(c->ctx, kernel, static_cast<int>((2 * total + 3) / 4), 128, static_cast<cudaStream_t>(stream), a);
 }
 
 }  // extern "C"

@@ -6,16 +6,16 @@
 #include "internal.hpp"
 
 namespace tb {
-// The attention kernel's maps and workspace (decode.cu), made with the cache.
+// The attention kernel's workspace, at the blob's start, and its maps (decode.cu).
+size_t decode_bytes(const tb_cache* c);
 tb_status decode_create(tb_cache* c);
-void decode_destroy(tb_cache* c);
 }  // namespace tb
 
 struct tb_cache {
     tb_context* ctx = nullptr;
     tb_cache_desc d{};
     tb_cache_buffers b{};
-    // Bookkeeping workspace (device), one allocation:
+    // Bookkeeping workspace (device), part of the blob:
     int32_t* marks = nullptr;    // [max_seqs] zero between calls: slots seen by the running call
     int32_t* offsets = nullptr;  // [max_seqs] first entry of each slot's new pages in `taken`
     int32_t* taken = nullptr;    // [num_pages] free pages found, lowest first

@@ -573,14 +573,18 @@ static int box_rows(int page_size) {  // the greatest common divisor of 64 and t
     return r;
 }
 
+static size_t part_places(const tb_cache* c) { return 4 * static_cast<size_t>(c->ctx->num_sms); }  // two a CTA
+
+size_t decode_bytes(const tb_cache* c) {
+    return part_places(c) * kUnitRows * (c->d.head_dim * sizeof(float) + sizeof(float2)) + part_places(c) / 2 * sizeof(uint32_t) * 4;
+}
+
 tb_status decode_create(tb_cache* c) {
     const tb_cache_desc& d = c->d;
     c->decode_ctas = 2 * c->ctx->num_sms;
-    const size_t places = 2 * static_cast<size_t>(c->decode_ctas);
-    TB_CUDA(cudaMalloc(&c->part_o, places * kUnitRows * d.head_dim * sizeof(float)));
-    TB_CUDA(cudaMalloc(&c->part_ml, places * kUnitRows * sizeof(float2)));
-    TB_CUDA(cudaMalloc(&c->arrived, c->decode_ctas * sizeof(uint32_t)));
-    TB_CUDA(cudaMemset(c->arrived, 0, c->decode_ctas * sizeof(uint32_t)));
+    c->part_o = static_cast<float*>(c->blob);
+    c->part_ml = reinterpret_cast<float2*>(c->part_o + part_places(c) * kUnitRows * d.head_dim);
+    c->arrived = reinterpret_cast<uint32_t*>(c->part_ml + part_places(c) * kUnitRows);
     const uint64_t rows = static_cast<uint64_t>(d.num_pages) * d.kv_heads * d.page_size;
     const uint64_t dims[2] = {static_cast<uint64_t>(d.head_dim), rows};
     const uint64_t stride[1] = {static_cast<uint64_t>(d.head_dim) * 2};
@@ -594,12 +598,6 @@ tb_status decode_create(tb_cache* c) {
         TB_TRY(encode_tiled(&c->v_map[l], type, 2, static_cast<const char*>(c->b.v_pages) + at, dims, stride, box, CU_TENSOR_MAP_SWIZZLE_128B));
     }
     return TB_OK;
-}
-
-void decode_destroy(tb_cache* c) {
-    if (c->part_o) cudaFree(c->part_o);
-    if (c->part_ml) cudaFree(c->part_ml);
-    if (c->arrived) cudaFree(c->arrived);
 }
 
 template <bool BF16, int DCH, int NT>
