@@ -95,7 +95,7 @@ def _check(dtype, q, k, v, lens, slots, scale, out, lse):
             assert not bad.any(), (i, s, lens[s], h, np.argwhere(bad)[:4], np.abs(out[i, hs] - want).max())
             none = np.isneginf(wlse)
             assert np.array_equal(np.isneginf(lse[i, hs]), none), (i, s, h)
-            assert (np.abs(lse[i, hs] - wlse)[~none] <= ltol[~none]).all(), (i, s, h)
+            assert (np.abs(lse[i, hs][~none] - wlse[~none]) <= ltol[~none]).all(), (i, s, h)
 
 
 ATTEND = [
@@ -534,3 +534,40 @@ def test_call_refusals(ctx):
     assert lib.tb_cache_free(c.h, L.ptr(one), -1, None) == L.TB_ERR_SHAPE_MISMATCH
     assert lib.tb_cache_compact(None, None, None, None) == L.TB_ERR_INVALID_ARGUMENT
     ctx.synchronize()
+
+
+def test_attend_many_rows(ctx):
+    """More rows than one look at their lengths takes (128), slots in any order and more than once."""
+    r = np.random.default_rng(20)
+    lens = [int(x) for x in r.choice([0, 1, 15, 16, 17, 64, 65, 200], 90)]
+    c, k, v = _filled(ctx, 21, "f16", lens, 1, 64, 16)
+    slots = [int(x) for x in r.integers(0, 90, 700)]
+    q = torch.randn(700, 3, 64, device="cuda").half()
+    out, lse = c.attend(0, _ints(slots), q)
+    ctx.synchronize()
+    _check("f16", q, k, v, lens, slots, np.float32(0.125), out, lse)
+
+
+def test_bookkeeping_of_more_slots_than_threads(ctx):
+    """1500 slots in one call, more pages than one pass over the counts takes (4096)."""
+    c = _cache(ctx, "bf16", 1, 9000, 8, 1, 16, 3000, 6)
+    m = A.Cache(9000, 8, 3000, 6)
+    r = np.random.default_rng(22)
+    slots = [int(x) for x in r.permutation(3000)[:1500]]
+    counts = [int(x) for x in r.integers(0, 40, 1500)]
+    assert m.reserve(slots, counts)
+    c.reserve(_ints(slots), _ints(counts))
+    ctx.synchronize()
+    _same(c, m)
+    children = [s for s in range(3000) if s not in set(slots)]
+    parents = [slots[int(x)] for x in r.integers(0, 1500, len(children))]
+    assert m.fork(parents, children) is not None
+    c.fork(_ints(parents), _ints(children))
+    ctx.synchronize()
+    _same(c, m)
+    m.free(slots)
+    c.free(_ints(slots))
+    m.compact()
+    c.compact()
+    ctx.synchronize()
+    _same(c, m)

@@ -286,6 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // The next kernel may be placed on the SMs that are free; it waits for this one before it reads anything.
+    if (threadIdx.x == 0) grid_launch_dependents();
     const uint32_t tmem = sh.tmem;
     const long long limit = a.timeout_cycles;
     const long long drain_limit = limit > kDrainCycles ? limit : kDrainCycles;
@@ -437,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 return x;
             };
+            const Seq first_window = look_at(lane);  // up to 32 sequences are looked at once
             for (int k = 0;; ++k) {
                 int valid = 0, q0s = 0, k0s = 0, lq = 0, lk = 0, sub = 0, kv_head = 0;
                 const long long want = block < 0 ? 0 : block / a.kv_heads;
@@ -449,14 +452,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (b0 >= a.batch) {  // the next lower level that occurs
                         int top = -1;
                         for (int b = lane; b < a.batch; b += 32) {
-                            const int l = look_at(b).level;
+                            const int l = (b < 32 ? first_window : look_at(b)).level;
                             if (l < level) top = max(top, l);
                         }
                         level = __reduce_max_sync(0xffffffffu, top);
                         if (level < 0) break;
                         b0 = 0;
                     }
-                    const Seq x = look_at(b0 + lane);
+                    const Seq x = b0 == 0 ? first_window : look_at(b0 + lane);
                     int n = x.level == level ? ((x.lq + kRows - 1) / kRows * a.group + 1) >> 1 : 0;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
