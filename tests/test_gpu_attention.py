@@ -360,3 +360,17 @@ def test_two_streams_at_once(ctx):
     torch.cuda.synchronize()
     for pair in sum(got, []):
         assert torch.equal(pair[0], want) and torch.equal(pair[1], wlse)
+
+
+@pytest.mark.parametrize("hq,hk", [(2, 1), (8, 2), (8, 1), (16, 1), (32, 1), (64, 1), (6, 1), (10, 2)])
+def test_heads_that_share_a_tile(ctx, hq, hk):
+    """Groups of a power of two share a tile's rows (up to 32 heads), others do not: tokens around a tile's and a warp's end."""
+    group = hq // hk
+    tokens = max(1, 128 // group)
+    lq = [1, tokens - 1, tokens, tokens + 1, 2 * tokens + 3, 0, 7]
+    lq = [max(n, 0) for n in lq]
+    lk = [n + 3 for n in lq]
+    q, k, v = _inputs(23 + hq, "bf16", lq, lk, hq, hk, 64)
+    out, lse = attention(ctx, q, k, v, _offsets(lq), _offsets(lk))
+    ctx.synchronize()
+    _check("bf16", q, k, v, lq, lk, True, np.float32(0.125), out, lse)

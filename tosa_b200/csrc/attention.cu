@@ -10,8 +10,10 @@
 // o are multiplied by 2^(m - m'). Weights stay below 2^13, far inside the range of both types, and
 // since weights and their sum share m the result does not depend on it. lse = (m + log2 l) ln 2.
 //
-// An item is two tiles of 128 rows (two heads of one key head's group, or two row tiles of one head) that
-// walk the same blocks of 128 keys. One CTA an SM takes item after item: the grid has a block for each,
+// A tile is 128 rows: 128 tokens of one head, or where the group of a key head is a power of two up to 32,
+// 128 / group tokens of all its heads (row = token * group + head), so that short sequences fill their
+// tiles (one token of 8 heads takes 8 rows of one tile instead of one row of 8). An item is two tiles of
+// one key head that walk the same blocks of 128 keys. One CTA an SM takes item after item: the grid has a block for each,
 // and a running CTA takes over blocks that have not begun, heaviest first within a sequence. 16 warps:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one row a thread: read the scores from tensor memory, write
 //                   the weights back to it as f16 / bf16, and rescale o there when m moves
@@ -39,7 +41,8 @@
 
 namespace tb {
 
-constexpr int kRows = 128;      // rows of a tile
+constexpr int kRowsLog = 7;
+constexpr int kRows = 1 << kRowsLog;  // rows of a tile
 constexpr int kKeys = 128;      // keys of a block
 constexpr int kThreads = 512;
 // Registers: launched with 128 a thread (65,536); the two softmax warpgroups take 192, the others keep 64.
@@ -71,9 +74,9 @@ struct PromptCfg {
 // A guarded value that is not finite is noted by its key, counted from the item's first guarded block.
 constexpr uint32_t kNoKey = 0xFFFFu;
 
-// One tile's place: rows row0 .. row0 + rows - 1 of its sequence, of one head.
+// One tile's place: its rows are the tokens from token0 on, each of the packed heads from `head` on.
 struct Tile {
-    int row0, rows, head;
+    int token0, rows, head;
     int blocks;       // blocks of keys that some row sees
     int seen_by_all;  // keys that every row sees (the first row's)
 };
@@ -106,6 +109,7 @@ struct PromptArgs {
     long long o_token, o_head;
     long long total_q, total_k;
     int batch, group, kv_heads, head_dim, causal;
+    int pack_log;             // log2 of the heads that share a tile
     float scale_log2;
     unsigned early_next;  // grids up to this size let the next kernel start early
     uint32_t* err;
@@ -116,19 +120,22 @@ __device__ __forceinline__ int visible(int causal, int row, int lq, int lk) {
     return causal ? max(0, min(lk, row + lk - lq + 1)) : lk;
 }
 
-// Tile `sub` of a key head's group, in the order (row tile, head of the group).
+// Tiles of a key head's group for lq tokens, and tile `sub` of them in the order (token, head).
+__device__ __forceinline__ int tiles_of(const PromptArgs& a, int lq) {
+    const int tokens_log = kRowsLog - a.pack_log;
+    return ((lq + (1 << tokens_log) - 1) >> tokens_log) * (a.group >> a.pack_log);
+}
 __device__ __forceinline__ Tile tile_of(const PromptArgs& a, int sub, int kv_head, int lq, int lk) {
     Tile x{0, 0, 0, 0, INT32_MAX};
-    const int rt = sub / a.group;
-    x.row0 = rt * kRows;
-    x.rows = min(kRows, lq - x.row0);
-    if (x.rows <= 0) {
-        x.rows = 0;
-        return x;
-    }
-    x.head = kv_head * a.group + (sub - rt * a.group);
-    x.blocks = (visible(a.causal, x.row0 + x.rows - 1, lq, lk) + kKeys - 1) / kKeys;
-    x.seen_by_all = visible(a.causal, x.row0, lq, lk);
+    const int heads = a.group >> a.pack_log;  // 1 where all of the group is packed
+    const int st = heads == 1 ? sub : sub / heads;
+    x.token0 = st << (kRowsLog - a.pack_log);
+    const int tokens = min(kRows >> a.pack_log, lq - x.token0);
+    if (tokens <= 0) return x;
+    x.rows = tokens << a.pack_log;
+    x.head = kv_head * a.group + ((sub - st * heads) << a.pack_log);
+    x.blocks = (visible(a.causal, x.token0 + tokens - 1, lq, lk) + kKeys - 1) / kKeys;
+    x.seen_by_all = visible(a.causal, x.token0, lq, lk);
     return x;
 }
 
@@ -334,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int t = 0; t < 2; ++t) {
                 const Tile my = it.tile[t];
                 if (my.rows == 0) continue;
-                const int sees = visible(a.causal, min(my.row0 + r, my.row0 + my.rows - 1), it.lq, it.lk);
+                const int sees = visible(a.causal, my.token0 + (min(r, my.rows - 1) >> a.pack_log), it.lq, it.lk);
                 const uint32_t to = tmem + (static_cast<uint32_t>(w * 32) << 16) + 256 + t * 128;
                 ok = wait(&sh.ml_full[t], outs[t]++ & 1);
                 if (ok && my.blocks > 0) ok = wait(&sh.guard_done[k % kItems], (k / kItems) & 1) && wait(&sh.o_full[t], prods[t]++ & 1);
@@ -349,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint16_t* first = reinterpret_cast<const uint16_t*>(&sh.first[k % kItems][0][0]);
                 const int rel = odd ? sees - it.first_guarded * kKeys : 0;
                 const bool whole = 32 * w + 32 <= my.rows;
-                const int token = it.q0 + my.row0 + 32 * w;
+                const int token = it.q0 + my.token0 + ((32 * w) >> a.pack_log);  // the warp's first (pack <= 32)
 #pragma unroll 1
                 for (int c0 = 0; c0 < a.head_dim; c0 += 64) {
                     if (lane == 0) bulk_wait_read0();  // the buffer's last store has left
@@ -401,14 +408,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     } else {
                         __syncwarp();
                         uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(token) * a.o_token + my.head * a.o_head + c0;
-                        const int v = lane & 7;
+                        const int v = lane & 7, pack = (1 << a.pack_log) - 1;
                         for (int rr = lane >> 3; 32 * w + rr < my.rows && rr < 32; rr += 4)
-                            if (c0 + 8 * v < a.head_dim) *reinterpret_cast<uint4*>(out + rr * a.o_token + 8 * v) = st[rr * 8 + (v ^ (rr & 7))];
+                            if (c0 + 8 * v < a.head_dim)
+                                *reinterpret_cast<uint4*>(out + (rr >> a.pack_log) * a.o_token + (rr & pack) * a.o_head + 8 * v) =
+                                    st[rr * 8 + (v ^ (rr & 7))];
                         __syncwarp();
                     }
                 }
                 if (a.lse != nullptr && r < my.rows)
-                    a.lse[static_cast<long long>(my.head) * a.total_q + token + lane] =
+                    a.lse[static_cast<long long>(my.head + (lane & ((1 << a.pack_log) - 1))) * a.total_q + token + (lane >> a.pack_log)] =
                         any && m != -INFINITY ? (m + __log2f(l)) * kLn2 : -INFINITY;
             }
             if (!ok) break;
@@ -425,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             RingPos r;
             uint32_t loads = 0, qn[2] = {0, 0};
             bool ok = true;
-            // Items lie sequence behind sequence, ceil(row tiles * group / 2) for each; sequences whose rows see
+            // Items lie sequence behind sequence, ceil(tiles / 2) for each; sequences whose rows see
             // many keys first (by the power of two of their blocks), so that no long item begins late.
             int level = 32, b0 = a.batch;  // sequences of this level before b0, and of higher levels, have
             long long before = 0;          // `before` items (items come in rising order, as a rule)
@@ -465,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         b0 = 0;
                     }
                     const Seq x = b0 == 0 ? first_window : look_at(b0 + lane);
-                    int n = x.level == level ? ((x.lq + kRows - 1) / kRows * a.group + 1) >> 1 : 0;
+                    int n = x.level == level ? (tiles_of(a, x.lq) + 1) >> 1 : 0;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
                         const int y = __shfl_up_sync(0xffffffffu, n, o);
@@ -562,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // Q's place is free only when the last item's last scores are through: until then its tiles come
                 // as far as L2, and the first K block goes ahead
                 if (lane < 2 * DCH && it.tile[lane / DCH].blocks)
-                    tma_prefetch_3d(&tmQ, 64 * (lane % DCH), it.tile[lane / DCH].head, q0s + it.tile[lane / DCH].row0);
+                    tma_prefetch_3d(&tmQ, 64 * (lane % DCH), it.tile[lane / DCH].head, q0s + it.tile[lane / DCH].token0);
                 __syncwarp();
                 if (blocks > 0) load_block(&tmK, 0);
                 for (int t = 0; t < 2 && ok; ++t) {
@@ -573,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         mbar_arrive_expect_tx(&sh.q_full[t], Cfg::kTile);
 #pragma unroll
                         for (int c = 0; c < DCH; ++c)
-                            tma_load_3d(sq + t * Cfg::kTile + c * Cfg::kChunk, &tmQ, &sh.q_full[t], 64 * c, it.tile[t].head, q0s + it.tile[t].row0);
+                            tma_load_3d(sq + t * Cfg::kTile + c * Cfg::kChunk, &tmQ, &sh.q_full[t], 64 * c, it.tile[t].head, q0s + it.tile[t].token0);
                     }
                     __syncwarp();
                     ++qn[t];
@@ -748,8 +757,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Tile my = it.tile[t];
             // keys that this thread's row sees, and the first and the last row of the warp (rows past the
             // tile's end count as its last)
-            const int last = my.row0 + my.rows - 1;
-            const int sees = visible(a.causal, min(my.row0 + r, last), it.lq, it.lk);
+            const int last = (my.rows - 1) >> a.pack_log;
+            const int sees = visible(a.causal, my.token0 + min(r >> a.pack_log, last), it.lq, it.lk);
             const int lo = __shfl_sync(0xffffffffu, sees, 0), hi = __shfl_sync(0xffffffffu, sees, 31);
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < my.blocks; ++j, ++n) {
@@ -886,14 +895,14 @@ tb_status attention_check(const char* op, int dtype, int q_heads, int kv_heads, 
     return TB_OK;
 }
 
-// [tokens][heads][head_dim] as {head_dim, heads, tokens}, boxes of some tokens by 64 elements of one head.
+// [tokens][heads][head_dim] as {head_dim, heads, tokens}, boxes of some tokens by some heads by 64 elements.
 static tb_status tile_map(CUtensorMap* m, const tb_attention_desc* d, const void* p, int64_t heads, int64_t tokens,
-                          int64_t token_stride, int64_t head_stride, int box_tokens = kRows) {
+                          int64_t token_stride, int64_t head_stride, int box_heads, int box_tokens) {
     // the stride of a dimension of one element says nothing; the map wants a valid one
     const uint64_t head = heads > 1 ? head_stride : d->head_dim, token = tokens > 1 ? token_stride : d->head_dim;
     const uint64_t dims[3] = {static_cast<uint64_t>(d->head_dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens)};
     const uint64_t strides[2] = {head * 2, token * 2};
-    const uint32_t box[3] = {64, 1, static_cast<uint32_t>(box_tokens)};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(box_heads), static_cast<uint32_t>(box_tokens)};
     return encode_tiled(m, d->dtype == TB_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p,
                         dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
@@ -956,21 +965,25 @@ TB_API tb_status tb_attention(tb_context* ctx, const tb_attention_desc* d, const
     // without keys nothing is loaded; the maps are made of q's first row
     const bool keys = d->total_k > 0;
     CUtensorMap mq, mk, mv, mo;
-    TB_TRY(tile_map(&mq, d, q, d->q_heads, d->total_q, d->q_token_stride, d->q_head_stride));
-    TB_TRY(tile_map(&mk, d, keys ? k : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->k_token_stride, d->k_head_stride));
-    TB_TRY(tile_map(&mv, d, keys ? v : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->v_token_stride, d->v_head_stride));
-    TB_TRY(tile_map(&mo, d, out, d->q_heads, d->total_q, d->out_token_stride, d->out_head_stride, 32));
     const int group = d->q_heads / d->kv_heads;
+    int pack = 0;  // log2 of the heads of a tile
+    if (group <= 32 && (group & (group - 1)) == 0)
+        while ((1 << pack) < group) ++pack;
+    TB_TRY(tile_map(&mq, d, q, d->q_heads, d->total_q, d->q_token_stride, d->q_head_stride, 1 << pack, kRows >> pack));
+    TB_TRY(tile_map(&mk, d, keys ? k : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->k_token_stride, d->k_head_stride, 1, kKeys));
+    TB_TRY(tile_map(&mv, d, keys ? v : q, keys ? d->kv_heads : 1, keys ? d->total_k : 1, d->v_token_stride, d->v_head_stride, 1, kKeys));
+    TB_TRY(tile_map(&mo, d, out, d->q_heads, d->total_q, d->out_token_stride, d->out_head_stride, 1 << pack, 32 >> pack));
     // A grid that leaves SMs free lets the next kernel set itself up there (back to back, one chat turn 9.8 -> 8.9
     // us). With more items than SMs the next kernel's blocks would take SMs from this one's end (24 packed
     // prompts 126 -> 136 us).
     const unsigned early = static_cast<unsigned>(ctx->num_sms / 2);
     PromptArgs a{out, lse, cu_q, cu_k, d->out_token_stride, d->out_head_stride, d->total_q, d->total_k, d->batch, group,
-                 d->kv_heads, d->head_dim, d->causal, d->scale * kLog2e, early, ctx->dev_err, ctx->timeout_cycles};
+                 d->kv_heads, d->head_dim, d->causal, pack, d->scale * kLog2e, early, ctx->dev_err, ctx->timeout_cycles};
     // most items that lengths summing to total_q can have: the lengths themselves are on the device
     const long long seqs = d->batch < d->total_q ? d->batch : d->total_q;
-    const long long tiles = (d->total_q - seqs) / kRows + seqs;
-    const long long grid = (group % 2 ? (tiles * group + seqs) / 2 : tiles * (group / 2)) * d->kv_heads;
+    const long long heads = group >> pack;
+    const long long tiles = ((d->total_q - seqs) / (kRows >> pack) + seqs) * heads;
+    const long long grid = (heads % 2 ? (tiles + seqs) / 2 : tiles / 2) * d->kv_heads;
     if (grid > INT32_MAX) return fail(TB_ERR_NOT_ACCELERATED, "attention: more than 2^31 tiles");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool wide = d->head_dim > 64;
