@@ -356,9 +356,12 @@ TB_API tb_status tb_attention(tb_context *ctx, const tb_attention_desc *desc, co
  * page ids passed below are DEVICE int32 arrays, so a step needs no host copy
  * and can be captured in a CUDA graph. Calls on one cache must not overlap on
  * the GPU (they share its state and workspace): use one stream, or order them.
- * Index arrays are checked on the device: a bad slot, page, length or a page
- * shortage leaves the state unchanged and is reported by the next
- * tb_synchronize (TB_ERR_INVALID_ARGUMENT / TB_ERR_OUT_OF_PAGES). */
+ * Index arrays are checked on the device and what is wrong with them is reported
+ * by the next tb_synchronize (TB_ERR_INVALID_ARGUMENT / TB_ERR_OUT_OF_PAGES):
+ * a refused tb_cache_reserve, _fork or _free leaves the state unchanged; a write
+ * to a place that the slot does not have, and a copy of a page that does not
+ * exist, are left out; a row of tb_cache_attend whose slot or length is wrong is
+ * not written, one with a bad page in its table has no defined result. */
 typedef struct tb_cache_desc {
     int32_t dtype;            /* TB_DT_BF16 / TB_DT_FP16 */
     int32_t layers, kv_heads, head_dim; /* head_dim: a multiple of 16 up to 128 */

@@ -88,7 +88,8 @@ class PagedCache:
         b = L.CacheBuffers(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), refs.data_ptr())
         h = ctypes.c_void_p()
         self.h = None
-        L.check(L.load().tb_cache_create(ctx.h, ctypes.byref(d), ctypes.byref(b), ctypes.byref(h)))
+        with torch.cuda.device(k_pages.device):
+            L.check(L.load().tb_cache_create(ctx.h, ctypes.byref(d), ctypes.byref(b), ctypes.byref(h)))
         self.h = h
 
     @classmethod

@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -42,7 +43,9 @@ struct Refused {};  // a Python exception is set
 
 // Calls the library with the interpreter unlocked (a launch can wait for room in the stream's queue).
 template <class F>
-void call(F f) {
+void call(at::Device device, F f) {
+    c10::OptionalDeviceGuard guard;
+    if (device.is_cuda()) guard.reset_device(device);
     PyThreadState* state = PyEval_SaveThread();
     const tb_status st = f();
     PyEval_RestoreThread(state);
@@ -207,7 +210,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                   hk.row_stride, hk.head_stride, hv.row_stride, hv.head_stride, ho.row_stride, ho.head_stride};
         auto* h = static_cast<tb_context*>(handle(op, a[0]));
         void* st = stream_of(a[10], device);
-        call([&] { return tb_attention(h, &d, hq.p, hk.p, hv.p, cq.p, ck.p, ho.p,
+        call(device, [&] { return tb_attention(h, &d, hq.p, hk.p, hv.p, cq.p, ck.p, ho.p,
                            static_cast<float*>(lse.data_ptr()), st); });
         return pair(out, lse);
     });
@@ -226,7 +229,7 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Heads v = heads(op, "v", tensor(op, "v", a[6]), pages.scalar_type(), device, k.rows, pages.size(2), pages.size(4));
         auto* h = static_cast<tb_cache*>(handle(op, a[0]));
         void* st = stream_of(a[7], device);
-        call([&] { return tb_cache_write(h, layer, slots.p, offsets.p, slots.n, k.rows, k.p, k.row_stride,
+        call(device, [&] { return tb_cache_write(h, layer, slots.p, offsets.p, slots.n, k.rows, k.p, k.row_stride,
                              k.head_stride, v.p, v.row_stride, v.head_stride, st); });
         return none();
     });
@@ -250,7 +253,7 @@ PyObject* cache_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor lse = sums(op, a[7], q.rows, q.heads, device);
         auto* h = static_cast<tb_cache*>(handle(op, a[0]));
         void* st = stream_of(a[8], device);
-        call([&] { return tb_cache_attend(h, layer, slots.p, slots.n, static_cast<int32_t>(q.heads), scale,
+        call(device, [&] { return tb_cache_attend(h, layer, slots.p, slots.n, static_cast<int32_t>(q.heads), scale,
                               q.p, q.row_stride, q.head_stride, ho.p, ho.row_stride, ho.head_stride,
                               static_cast<float*>(lse.data_ptr()), st); });
         return pair(out, lse);
@@ -266,7 +269,7 @@ PyObject* cache_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int32_t* counts = a[3] == Py_None ? nullptr : index(op, "counts", a[3], device, slots.n).p;
         auto* h = static_cast<tb_cache*>(handle(op, a[0]));
         void* st = stream_of(a[4], device);
-        call([&] { return tb_cache_reserve(h, slots.p, counts, slots.n, st); });
+        call(device, [&] { return tb_cache_reserve(h, slots.p, counts, slots.n, st); });
         return none();
     });
 }
@@ -279,7 +282,7 @@ PyObject* cache_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Index slots = index(op, "slots", a[2], device);
         auto* h = static_cast<tb_cache*>(handle(op, a[0]));
         void* st = stream_of(a[3], device);
-        call([&] { return tb_cache_free(h, slots.p, slots.n, st); });
+        call(device, [&] { return tb_cache_free(h, slots.p, slots.n, st); });
         return none();
     });
 }
@@ -293,7 +296,7 @@ PyObject* cache_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Index children = index(op, "children", a[3], device, parents.n);
         auto* h = static_cast<tb_cache*>(handle(op, a[0]));
         void* st = stream_of(a[4], device);
-        call([&] { return tb_cache_fork(h, parents.p, children.p, parents.n, st); });
+        call(device, [&] { return tb_cache_fork(h, parents.p, children.p, parents.n, st); });
         return none();
     });
 }
@@ -307,7 +310,7 @@ PyObject* cache_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Index dst = index(op, "dst", a[3], device, src.n);
         auto* h = static_cast<tb_cache*>(handle(op, a[0]));
         void* st = stream_of(a[4], device);
-        call([&] { return tb_cache_copy_pages(h, src.p, dst.p, src.n, st); });
+        call(device, [&] { return tb_cache_copy_pages(h, src.p, dst.p, src.n, st); });
         return none();
     });
 }
@@ -328,7 +331,7 @@ PyObject* cache_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         auto* h = static_cast<tb_cache*>(handle(op, a[0]));
         void* st = stream_of(a[5], device);
-        call([&] { return tb_cache_compact(h, to[0], to[1], st); });
+        call(device, [&] { return tb_cache_compact(h, to[0], to[1], st); });
         return none();
     });
 }
