@@ -439,6 +439,7 @@ TB_API void tb_context_destroy(tb_context* ctx) {
     cudaSetDevice(ctx->device);
     if (ctx->dev_err) cudaFree(ctx->dev_err);
     if (ctx->trace) cudaFree(ctx->trace);
+    if (ctx->pool) cudaMemPoolDestroy(ctx->pool);  // workspaces still in use are freed with their caches
     delete ctx;
 }
 

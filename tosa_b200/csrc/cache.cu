@@ -513,6 +513,25 @@ static tb_status launch(tb_context* ctx, void (*kernel)(P...), int grid, int blo
     return TB_OK;
 }
 
+// Workspaces come from a pool of the context that keeps up to 64 MB of what was freed: mapping 5 MB anew for
+// each cache and unmapping it took 0.5 to 1.5 ms.
+static cudaError_t workspace_alloc(tb_context* ctx, size_t bytes, void** out) {
+    if (!ctx->pool) {
+        cudaMemPoolProps props = {};
+        props.allocType = cudaMemAllocationTypePinned;
+        props.location.type = cudaMemLocationTypeDevice;
+        props.location.id = ctx->device;
+        cudaError_t e = cudaMemPoolCreate(&ctx->pool, &props);
+        if (e != cudaSuccess) {
+            ctx->pool = nullptr;
+            return e;
+        }
+        uint64_t keep = 64u << 20;
+        cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep);
+    }
+    return cudaMallocFromPoolAsync(out, bytes, ctx->pool, nullptr);
+}
+
 static CopyArgs copy_args(const tb_cache* c) {
     CopyArgs a{};
     a.k = static_cast<uint4*>(c->b.k_pages);
@@ -575,7 +594,7 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
     // one allocation: the attention's workspace (16-byte pieces first), then the words that begin as zero
     const size_t words = 2 * static_cast<size_t>(d->max_seqs) + 5 * static_cast<size_t>(d->num_pages) + 4;
     const size_t parts = decode_bytes(c);
-    cudaError_t e = cudaMalloc(&c->blob, parts + words * sizeof(int32_t));
+    cudaError_t e = workspace_alloc(ctx, parts + words * sizeof(int32_t), &c->blob);
     if (e == cudaSuccess) e = cudaMemsetAsync(c->blob, 0, parts + words * sizeof(int32_t), nullptr);
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // other streams may be the first to use it
     if (e != cudaSuccess) {
@@ -607,7 +626,10 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
 
 TB_API void tb_cache_destroy(tb_cache* c) {
     if (!c) return;
-    if (c->blob) cudaFree(c->blob);
+    if (c->blob) {
+        cudaDeviceSynchronize();  // the workspace may go to another cache at once: calls on any stream are through
+        cudaFreeAsync(c->blob, nullptr);
+    }
     delete c;
 }
 

@@ -25,6 +25,7 @@ struct tb_context {
     uint32_t* dev_err = nullptr;     // device error word (DEV_ERR_* bits)
     long long timeout_cycles = 0;    // bound on every in-kernel wait
     uint64_t launches = 0;
+    cudaMemPool_t pool = nullptr;    // the caches' workspaces (made with the first one)
     long long* trace = nullptr;      // optional GEMM timeline buffer (TB_TRACE=1, TB_GEMM_TRACE builds)
     int epi_groups = -1;             // TB_GEMM_EPI_GROUPS: 0 / 1 force the GEMM epilogue form, -1 by tile count
 };
