@@ -548,6 +548,20 @@ def test_attend_many_rows(ctx):
     _check("f16", q, k, v, lens, slots, np.float32(0.125), out, lse)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,d,page", [(16, 1, 64, 8), (32, 2, 32, 24), (5, 1, 16, 64), (10, 1, 48, 128)])
+def test_attend_narrow_heads_many_tiles(ctx, dtype, hq, hk, d, page):
+    """Several tiles a CTA, an even and an odd number of them, that end anywhere in the last one or two."""
+    r = np.random.default_rng(hq + d)
+    lens = [int(x) for x in r.choice([64, 65, 127, 128, 129, 190, 191, 192, 193, 255, 257, 640, 1111, 2049], 40)]
+    c, k, v = _filled(ctx, 31, dtype, lens, hk, d, page)
+    slots = [int(x) for x in r.integers(0, 40, 200)]
+    q = torch.randn(200, hq, d, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(DT[dtype])
+    out, lse = c.attend(0, _ints(slots), q)
+    ctx.synchronize()
+    _check(dtype, q, k, v, lens, slots, np.float32(1 / math.sqrt(d)), out, lse)
+
+
 def test_bookkeeping_of_more_slots_than_threads(ctx):
     """1500 slots in one call, more pages than one pass over the counts takes (4096)."""
     c = _cache(ctx, "bf16", 1, 9000, 8, 1, 16, 3000, 6)

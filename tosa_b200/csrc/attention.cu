@@ -5,16 +5,16 @@
 // With t_j = scale * log2(e) * q_i.k_j the kernel keeps, per row, a reference m and
 // l = sum 2^(t_j - m), o = sum 2^(t_j - m) v_j. m is the maximum of the first 32 keys (of the first
 // block, where the row does not see all of it) and stays while the weights it gives are small enough: a
-// block's maximum is not looked for, the sums of its weights (which are
-// needed anyway) tell when it has run away, and then the block is done again with its maximum and l and
-// o are multiplied by 2^(m - m'). Weights stay below 2^13, far inside the range of both types, and
+// block's maximum is not looked for, the sums of its weights (which are needed anyway) tell when it has run
+// away, and then the block is done again with its maximum and l and o are multiplied by 2^(m - m'). Weights stay below 2^13, far inside the range of both types, and
 // since weights and their sum share m the result does not depend on it. lse = (m + log2 l) ln 2.
 //
 // A tile is 128 rows: 128 tokens of one head, or where the group of a key head is a power of two up to 32,
 // 128 / group tokens of all its heads (row = token * group + head), so that short sequences fill their
 // tiles (one token of 8 heads takes 8 rows of one tile instead of one row of 8). An item is two tiles of
-// one key head that walk the same blocks of 128 keys. One CTA an SM takes item after item: the grid has a block for each,
-// and a running CTA takes over blocks that have not begun, heaviest first within a sequence. 16 warps:
+// one key head that walk the same blocks of 128 keys. One CTA an SM takes item after item: the grid has a
+// block for each, and a running CTA takes over blocks that have not begun, sequences with many keys first
+// and the heaviest first within a sequence. 16 warps:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one row a thread: read the scores from tensor memory, write
 //                   the weights back to it as f16 / bf16, and rescale o there when m moves
 //   warp 8          issues the MMAs: S = Q K^T (both from shared memory), O += P V (P from tensor memory)

@@ -5,11 +5,11 @@
 // every SM streams the same amount, and the arithmetic only has to keep up. Keys and dimensions take
 // the long side of mma.sync's 16 x 8 x 16 and the query rows the short one, so at most 7 rows are padding.
 //
-// Cut: a unit is one sequence, key head and at most 8 (for groups above 8: 16) of its query heads; its keys come in tiles of 64
-// tokens. The tiles of all units in a row are divided evenly over the CTAs (two on each SM), so a CTA
-// takes the end of one unit, some whole units and the beginning of another. A unit that lies in one CTA
-// is finished there. Of a unit that several CTAs share, each leaves its unscaled sum, maximum and sum of
-// weights, and the CTA that arrives last adds them in the order of the keys: the result does not depend
+// Cut: a unit is one sequence, key head and at most 8 (for groups above 8: 16) of its query heads; its keys
+// come in tiles of 64 tokens. The tiles of all units in a row are divided evenly over the CTAs (two on each
+// SM), so a CTA takes the end of one unit, some whole units and the beginning of another. A unit that lies in
+// one CTA is finished there. Of a unit that several CTAs share, each leaves its unscaled sum, maximum and sum
+// of weights, and the CTA that arrives last adds them in the order of the keys: the result does not depend
 // on who that is. (It does depend, in its last bits, on where the cuts fall, that is on the lengths of the
 // whole batch.) Nobody waits for another CTA.
 //
@@ -19,16 +19,20 @@
 // maximum and the weights through shared memory, and take a quarter of head_dim each for
 // O^T += V^T P^T: two barriers a tile, and nothing to join among the warps when the CTA leaves a unit
 // (warps with a maximum and a result of their own need no barriers, but joining them made 32 contexts
-// of up to 1023 tokens of 32 heads 29.6 us instead of 24.7).
+// of up to 1023 tokens of 32 heads 29.6 us instead of 24.7). Tiles of heads of at most 64 are half as large
+// and share two barriers in pairs while a CTA's part of a unit has two (98 contexts of 5678 tokens, one head:
+// 34.2 -> 31.5 us; 8 of 4000 to 20000, 16 heads to each of 4 key heads: 29.6 -> 26.9). Tiles of 128 keys
+// instead cut short contexts too coarsely (40 of up to 300 tokens 7.3 -> 7.9 us).
 //
-// Measured: 64 contexts of up to 16384 tokens (8 key heads of 128, 1.66 GB) 248 us = 6.7 TB/s; two of 20 to 30
-// thousand (216 MB) 43.5 us = 5.0 TB/s, of which some 15 us are the start's dependent accesses (slot, length,
-// page, first tile) and the join of 37 parts a unit; the 32 short ones (73 MB) 22.2 us, bound by the
-// latency of the 4.5 units that a CTA goes through.
+// Measured: 64 contexts of up to 16384 tokens (8 key heads of 128, 1.66 GB) 247 us = 6.7 TB/s; two of 20 to 30
+// thousand (216 MB) 43.6 us = 5.0 TB/s: of some 63,000 cycles of a CTA its first tile's arrival takes 9,500 (slot,
+// length, page, tile one after the other) and its result 3,000; the 32 short ones (73 MB) 22.2 us, bound by the
+// latency of the units that a CTA goes through (one of two tiles takes some 6,000 cycles).
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "cache.hpp"
@@ -42,7 +46,6 @@ constexpr int kUnitRows = 16;                  // query rows of a unit at most
 constexpr int kConsumers = 128;
 constexpr int kDecodeThreads = kConsumers + 32;
 constexpr int kQPitch = 272;                   // bytes from one query row to the next: 8 rows hit 8 bank groups
-constexpr int kPPitch = 144;                   // bytes of one row of weights: 8 rows hit 8 bank groups
 constexpr long long kDecodeDrain = 2000000000ll;  // bound on a CTA's waits for its own copies at its end
 
 template <int DCH>
@@ -50,6 +53,8 @@ struct DecodeCfg {
     static constexpr int kTensor = DCH * kTokens * 128;  // K or V of a tile, 64-element chunks of 128-byte rows, swizzled
     static constexpr int kStage = 2 * kTensor;
     static constexpr int kStages = DCH == 2 ? 3 : 6;
+    static constexpr int kAtOnce = DCH == 2 ? 1 : 2;     // tiles between two barriers at most
+    static constexpr int kPPitch = kAtOnce * kTokens * 2 + 16;  // bytes of one row of weights: 8 rows hit 8 bank groups
     static constexpr int kSmem = 1024 + kStages * kStage + kUnitRows * kQPitch + kUnitRows * kPPitch;
 };
 
@@ -134,7 +139,7 @@ template <bool BF16, int DCH, int NT>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
     decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs a) {
     using Cfg = DecodeCfg<DCH>;
-    constexpr int S = Cfg::kStages;
+    constexpr int S = Cfg::kStages, kPPitch = Cfg::kPPitch;
     extern __shared__ uint8_t raw[];
     __shared__ DecodeShared sh;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -355,15 +360,22 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
                 m[h][e] = -INFINITY;
                 l[h][e] = 0.f;
             }
-        for (int t = walk.t0; t < walk.t1; ++t, ++it) {
-            const int s = it % S;
-            const uint32_t kb = smem_u32(ring + s * Cfg::kStage), vb = kb + Cfg::kTensor;
-            wait(&sh.full[s], (it / S) & 1);
-            const int live = walk.len - t * kTokens;  // keys of the tile that exist
-            float c[NT][4] = {}, d[NT][4] = {};
-            {
+        // `tiles` tiles of the ring from tile t on
+        auto step = [&](int t, auto tiles) {
+            constexpr int T = decltype(tiles)::value;
+            uint32_t kb[T];
+#pragma unroll
+            for (int u = 0; u < T; ++u) {
+                const int s = (it + u) % S;
+                kb[u] = smem_u32(ring + s * Cfg::kStage);
+                wait(&sh.full[s], ((it + u) / S) & 1);
+            }
+            const int live = walk.len - t * kTokens;  // keys from the first tile's start that exist
+            float c[NT][T][4] = {}, d[NT][T][4] = {};
+#pragma unroll
+            for (int u = 0; u < T; ++u) {
                 const int tok = 16 * warp + (mat & 1) * 8 + mrow;
-                const uint32_t ka = kb + tok * 128;
+                const uint32_t ka = kb[u] + tok * 128;
 #pragma unroll
                 for (int k = 0; k < 4 * DCH; ++k) {
                     if (k < ksteps) {
@@ -372,18 +384,25 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
                         ldmatrix_x4(ka + (k >> 2) * (kTokens * 128) + ((v ^ (tok & 7)) << 4), x);
                         // (even and odd steps in sums of their own: half the chain)
 #pragma unroll
-                        for (int h = 0; h < NT; ++h) mma_16816<BF16>(k & 1 ? d[h] : c[h], x, qf[h][k][0], qf[h][k][1]);
+                        for (int h = 0; h < NT; ++h) mma_16816<BF16>(k & 1 ? d[h][u] : c[h][u], x, qf[h][k][0], qf[h][k][1]);
                     }
                 }
             }
 #pragma unroll
             for (int h = 0; h < NT; ++h) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    c[h][e] += d[h][e];
-                    if (16 * warp + r0 + (e & 2) * 4 >= live) c[h][e] = -INFINITY;
+                for (int u = 0; u < T; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        c[h][u][e] += d[h][u][e];
+                        if (kTokens * u + 16 * warp + r0 + (e & 2) * 4 >= live) c[h][u][e] = -INFINITY;
+                    }
+                float top[2] = {fmaxf(c[h][0][0], c[h][0][2]), fmaxf(c[h][0][1], c[h][0][3])};
+#pragma unroll
+                for (int u = 1; u < T; ++u) {
+                    top[0] = fmaxf(top[0], fmaxf(c[h][u][0], c[h][u][2]));
+                    top[1] = fmaxf(top[1], fmaxf(c[h][u][1], c[h][u][3]));
                 }
-                float top[2] = {fmaxf(c[h][0], c[h][2]), fmaxf(c[h][1], c[h][3])};
 #pragma unroll
                 for (int i = 4; i < 32; i *= 2) {
                     top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], i));
@@ -404,31 +423,39 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
                     const float mm = fmaxf(m[h][e], top[e]), b = mm == -INFINITY ? 0.f : mm;
                     const float f = exp2_fast(m[h][e] - b);
                     m[h][e] = mm;
-                    c[h][e] = exp2_fast(fmaf(c[h][e], a.scale_log2, -b));
-                    c[h][e + 2] = exp2_fast(fmaf(c[h][e + 2], a.scale_log2, -b));
-                    l[h][e] = l[h][e] * f + c[h][e] + c[h][e + 2];
+                    l[h][e] *= f;
+#pragma unroll
+                    for (int u = 0; u < T; ++u) {
+                        c[h][u][e] = exp2_fast(fmaf(c[h][u][e], a.scale_log2, -b));
+                        c[h][u][e + 2] = exp2_fast(fmaf(c[h][u][e + 2], a.scale_log2, -b));
+                        l[h][e] = l[h][e] + c[h][u][e] + c[h][u][e + 2];
+                    }
 #pragma unroll
                     for (int i = 0; i < DCH; ++i) {
                         o[i][h][e] *= f;
                         o[i][h][e + 2] *= f;
                     }
                 }
-                // the weights by rows, 16 of this warp's keys
-                uint8_t* pw = sp + (8 * h + r0) * kPPitch + (16 * warp + cpair) * 2;
-                *reinterpret_cast<uint32_t*>(pw) = movmatrix_trans(pack2<BF16>(c[h][0], c[h][1]));
-                *reinterpret_cast<uint32_t*>(pw + 16) = movmatrix_trans(pack2<BF16>(c[h][2], c[h][3]));
+                // the weights by rows, 16 of this warp's keys a tile
+#pragma unroll
+                for (int u = 0; u < T; ++u) {
+                    uint8_t* pw = sp + (8 * h + r0) * kPPitch + (kTokens * u + 16 * warp + cpair) * 2;
+                    *reinterpret_cast<uint32_t*>(pw) = movmatrix_trans(pack2<BF16>(c[h][u][0], c[h][u][1]));
+                    *reinterpret_cast<uint32_t*>(pw + 16) = movmatrix_trans(pack2<BF16>(c[h][u][2], c[h][u][3]));
+                }
             }
             consumer_sync();
-            // O^T += V^T P^T over all 64 keys, this warp's part of head_dim
+            // O^T += V^T P^T over all keys, this warp's part of head_dim
             const uint32_t pa = smem_u32(sp) + mrow * kPPitch + mat * 16;
 #pragma unroll
-            for (int k = 0; k < kTokens / 16; k += 2) {
+            for (int k = 0; k < T * kTokens / 16; k += 2) {
+                const uint32_t vb = kb[k / (kTokens / 16)] + Cfg::kTensor;
                 uint32_t p[NT][4];
 #pragma unroll
                 for (int h = 0; h < NT; ++h) ldmatrix_x4(pa + 8 * h * kPPitch + k * 32, p[h]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int tok = 16 * (k + j) + (mat >> 1) * 8 + mrow;
+                    const int tok = 16 * ((k + j) % (kTokens / 16)) + (mat >> 1) * 8 + mrow;
                     // keys past the end have weight 0, but what lies in their place may be NaN
                     const int left = live - 16 * (k + j) - cpair;
                     const uint32_t lo = left >= 2 ? 0xFFFFFFFFu : (left == 1 ? 0x0000FFFFu : 0u);
@@ -451,8 +478,16 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.empty[s]);
-        }
+            if (lane == 0) {
+#pragma unroll
+                for (int u = 0; u < T; ++u) mbar_arrive(&sh.empty[(it + u) % S]);
+            }
+            it += T;
+        };
+        int t = walk.t0;
+        if constexpr (Cfg::kAtOnce == 2)
+            for (; t + 2 <= walk.t1; t += 2) step(t, std::integral_constant<int, 2>());
+        for (; t < walk.t1; ++t) step(t, std::integral_constant<int, 1>());
         // ---------------------------------------------------------------- the unit's end
 #pragma unroll
         for (int h = 0; h < NT; ++h)
