@@ -34,8 +34,8 @@
 // 456 in short runs and 524 instead of 518 in sustained ones: the softmax is bound by the instructions
 // that one warp can issue, and in sustained runs by power.)
 //
-// Measured at head_dim 128, bf16: 8192 causal rows of 32 heads in 474 us, 1160 TFLOP/s, in sustained runs at the
-// power cap (1.46 GHz), 418 us, 1315 TFLOP/s, in short ones; tensor pipe 68 % and special-function units
+// Measured at head_dim 128, bf16: 8192 causal rows of 32 heads in 476 us, 1155 TFLOP/s, in sustained runs at the
+// power cap (1.46 GHz), 411 us, 1338 TFLOP/s, in short ones; tensor pipe 68 % and special-function units
 // 67 % of the active cycles. A block of both tiles takes some 2850 cycles, 2048 of them MMAs.
 #include <cuda_runtime.h>
 
