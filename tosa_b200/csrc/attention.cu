@@ -34,9 +34,9 @@
 // 456 in short runs and 524 instead of 518 in sustained ones: the softmax is bound by the instructions
 // that one warp can issue, and in sustained runs by power.)
 //
-// Measured at head_dim 128, bf16: 8192 causal rows of 32 heads in 476 us, 1155 TFLOP/s, in sustained runs at the
-// power cap (1.46 GHz), 411 us, 1338 TFLOP/s, in short ones; tensor pipe 68 % and special-function units
-// 67 % of the active cycles. A block of both tiles takes some 2850 cycles, 2048 of them MMAs.
+// Measured at head_dim 128, bf16: 8192 causal rows of 32 heads in 476 to 490 us by the machine, 1122 to 1155
+// TFLOP/s, in sustained runs at the power cap (1.46 GHz), 410 to 421 us, 1306 to 1341 TFLOP/s, in short ones;
+// tensor pipe 68 % and special-function units 67 % of the active cycles. A block of both tiles takes some 2850 cycles, 2048 of them MMAs.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -771,7 +771,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < my.blocks; ++j, ++n) {
                 ok = wait(&sh.s_full[t], n & 1);
                 if (!ok) break;
-                //TR(warp)
                 tc_fence_after();
                 uint32_t s[128];
 #pragma unroll
@@ -783,7 +782,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     asm volatile("" : "+r"(s[i]));
                     x[i] = __uint_as_float(s[i]);
                 }
-                //TR(8+warp)
                 const int lo_j = lo - j * kKeys, hi_j = hi - j * kKeys;
                 // O and l to a new reference. (O holds every product so far: S was committed after them.)
                 auto rescale = [&](float to_m) {
@@ -868,7 +866,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     hand_over(&sh.p_full[t]);
                 }
-                //TR(32+warp)
             }
             if (!ok) break;
             if (my.rows > 0) {

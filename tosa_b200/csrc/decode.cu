@@ -256,10 +256,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
             const int head = walk.unit / a.chunks, chunk = walk.unit - head * a.chunks;
             const int rows = min(8 * NT, a.group - chunk * 8 * NT);
             const int32_t* table = a.table + static_cast<long long>(walk.slot) * a.max_pages;
-            // lane p < pieces loads piece p of every tile; its page is looked up one tile ahead
+            // lane p < pieces loads piece p of every tile; its page and its place there are found one tile ahead (one
+            // division for both: pages of 8 tokens 40.2 -> 39.0 us, though 16 contexts in pages of 16 20.3 -> 20.7)
+            int inside = 0;  // the piece's first token in its page
             auto lookup = [&](int t) {
                 const int tok = t * kTokens + lane * a.box;
-                return lane < pieces && tok < walk.len ? table[tok / a.page_size] : -1;
+                const int at = tok / a.page_size;
+                inside = tok - at * a.page_size;
+                return lane < pieces && tok < walk.len ? table[at] : -1;
             };
             int page = lookup(walk.t0);
             const int qs = seg & (q_slots - 1);
@@ -284,13 +288,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
                 if (lane == 0) mbar_arrive_expect_tx(&sh.full[s], count * a.box * 256 * DCH);
                 __syncwarp();
                 int p = page;
+                const int row0 = inside;
                 if (mine && (p < 0 || p >= a.num_pages)) {  // refused, but the copies that were announced are made
                     atomicOr(a.err, DEV_ERR_INDEX);
                     p = 0;
                 }
                 if (t + 1 < walk.t1) page = lookup(t + 1);
                 if (mine) {
-                    const int row = (p * a.kv_heads + head) * a.page_size + tok % a.page_size;
+                    const int row = (p * a.kv_heads + head) * a.page_size + row0;
                     uint8_t* k = ring + s * Cfg::kStage + lane * a.box * 128;
 #pragma unroll
                     for (int c = 0; c < DCH; ++c) {
