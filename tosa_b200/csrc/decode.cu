@@ -520,7 +520,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
                 inv[e] = walk.len > 0 ? __fdividef(1.f, sum) : 0.f;
                 if (warp == 0 && r0 == 0 && row < rows) {
                     if (!whole) a.part_ml[place * kUnitRows + row] = make_float2(m[h][e], sum);
-                    else if (lse != nullptr) lse[row] = m[h][e] == -INFINITY ? -INFINITY : (m[h][e] + __log2f(sum)) * kLn2;
+                    // (no key: -inf + log 0. The maximum passes over scores of NaN, their sum does not)
+                    else if (lse != nullptr) lse[row] = (m[h][e] + __log2f(sum)) * kLn2;
                 }
             }
 #pragma unroll
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
                 const float inv = __fdividef(1.f, ll);  // (a unit in parts has tokens)
                 *reinterpret_cast<uint2*>(out + row * a.o_head + 4 * v) =
                     make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
-                if (lse != nullptr && v == 0) lse[row] = mm == -INFINITY ? -INFINITY : (mm + __log2f(ll)) * kLn2;
+                if (lse != nullptr && v == 0) lse[row] = (mm + __log2f(ll)) * kLn2;
             }
         }
     }
