@@ -63,3 +63,48 @@ def test_scores_of_nan_make_the_rows_sum_nan(ctx, lens, where, d):
     assert torch.isnan(out[1, :4]).all() and torch.isnan(lse[1, :4]).all()
     assert torch.equal(out[1, 4:], want[1, 4:]) and torch.equal(lse[1, 4:], wlse[1, 4:])
     assert torch.equal(out[[0, 2]], want[[0, 2]]) and torch.equal(lse[[0, 2]], wlse[[0, 2]])
+
+
+def _busy(tensor):
+    """Work on the current stream that lasts some milliseconds and then writes all of `tensor`."""
+    x = torch.ones(1 << 28, device="cuda")
+    for _ in range(20):
+        x.add_(1.0)
+    tensor.fill_(7.0)
+
+
+@pytest.mark.parametrize("op", ["prompt", "token"])
+def test_results_on_another_stream_are_not_memory_in_use(ctx, op):
+    """A block that was freed while work queued on the caller's stream still writes it is no place for results that
+    another stream writes at once."""
+    if op == "prompt":
+        q, k, v = (torch.randn(2048, h, 128, device="cuda").bfloat16() for h in (8, 2, 2))
+        cu = _offsets([2048])
+        call = lambda **kw: attention(ctx, q, k, v, cu, cu, **kw)  # noqa: E731
+    else:
+        c, slots, q, k, v = _filled(ctx, [200 + i for i in range(256)], 2, 128)
+        call = lambda **kw: c.attend(0, slots, q, **kw)  # noqa: E731
+    want, wlse = call()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for one in (want, wlse):
+        last = torch.empty_like(one)
+        place = last.data_ptr()
+        _busy(last)
+        del last
+        out, lse = call(stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, wlse)
+        assert place not in (out.data_ptr(), lse.data_ptr())
+
+
+def test_results_given_by_the_caller_are_used_on_another_stream(ctx):
+    q, k, v = (torch.randn(300, h, 64, device="cuda").bfloat16() for h in (4, 2, 2))
+    cu = _offsets([300])
+    want, wlse = attention(ctx, q, k, v, cu, cu)
+    out, lse = torch.zeros_like(want), torch.zeros_like(wlse)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = attention(ctx, q, k, v, cu, cu, out=out, lse=lse, stream=side)
+    side.synchronize()
+    assert got[0] is out and got[1] is lse and torch.equal(out, want) and torch.equal(lse, wlse)

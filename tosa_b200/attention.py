@@ -44,15 +44,26 @@ def _hold(stream, *tensors):
             t.record_stream(stream)
 
 
+def _results_on(stream, call, *tensors):
+    """The results of `call`, allocated with `stream` current: a block of the caller's stream may still be in use there
+    by work queued before it was freed, and nothing orders that work with `stream`. The results are held for the
+    caller's stream, where they are used next."""
+    caller = torch.cuda.current_stream(stream.device)
+    with torch.cuda.stream(stream):
+        results = call(stream.cuda_stream)
+    _hold(stream, *tensors, *results)
+    _hold(caller, *results)
+    return results
+
+
 def attention(ctx, q, k, v, cu_q, cu_k, *, causal=True, scale=None, out=None, lse=None, stream=None):
     """Attention of packed sequences (tb_attention): q [total_q, q_heads, head_dim], k and v
     [total_k, kv_heads, head_dim], cu_q and cu_k int32 offsets of batch + 1. Returns (out, lse), out
     like q, lse float32 [q_heads, total_q]. `scale` defaults to 1 / sqrt(head_dim)."""
     if stream is None:
         return _native.attention(ctx, q, k, v, cu_q, cu_k, causal, scale, out, lse, None)
-    out, lse = _native.attention(ctx, q, k, v, cu_q, cu_k, causal, scale, out, lse, stream.cuda_stream)
-    _hold(stream, q, k, v, cu_q, cu_k, out, lse)
-    return out, lse
+    return _results_on(stream, lambda s: _native.attention(ctx, q, k, v, cu_q, cu_k, causal, scale, out, lse, s),
+                       q, k, v, cu_q, cu_k)
 
 
 class PagedCache:
@@ -133,9 +144,8 @@ class PagedCache:
         lse float32 [n, q_heads]."""
         if stream is None:
             return _native.cache_attend(self, self.k_pages, layer, slots, q, scale, out, lse, None)
-        out, lse = _native.cache_attend(self, self.k_pages, layer, slots, q, scale, out, lse, stream.cuda_stream)
-        _hold(stream, slots, q, out, lse)
-        return out, lse
+        return _results_on(stream, lambda s: _native.cache_attend(self, self.k_pages, layer, slots, q, scale, out, lse, s),
+                           slots, q)
 
     def fork(self, parents, children, *, stream=None):
         """children[i] becomes a copy of parents[i]; full pages are shared."""
