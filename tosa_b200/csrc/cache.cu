@@ -589,6 +589,7 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
     tb_cache* c = new (std::nothrow) tb_cache;
     if (!c) return fail(TB_ERR_INVALID_ARGUMENT, "cache: out of host memory");
     c->ctx = ctx;
+    c->device = ctx->device;
     c->d = *d;
     c->b = *b;
     // one allocation: the attention's workspace (16-byte pieces first), then the words that begin as zero
@@ -627,8 +628,12 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
 TB_API void tb_cache_destroy(tb_cache* c) {
     if (!c) return;
     if (c->blob) {
+        int current = c->device;
+        cudaGetDevice(&current);
+        if (current != c->device) cudaSetDevice(c->device);
         cudaDeviceSynchronize();  // the workspace may go to another cache at once: calls on any stream are through
         cudaFreeAsync(c->blob, nullptr);
+        if (current != c->device) cudaSetDevice(current);
     }
     delete c;
 }

@@ -13,6 +13,7 @@ tb_status decode_create(tb_cache* c);
 
 struct tb_cache {
     tb_context* ctx = nullptr;
+    int device = 0;  // the context's, which may be gone when the cache is destroyed
     tb_cache_desc d{};
     tb_cache_buffers b{};
     // Bookkeeping workspace (device), part of the blob:
