@@ -376,7 +376,8 @@ typedef struct tb_cache tb_cache;
 TB_API tb_status tb_cache_create(tb_context *ctx, const tb_cache_desc *desc, const tb_cache_buffers *buffers,
                                  tb_cache **out);
 /* Waits for the work of the cache's device, whichever is current, before it frees the
- * workspace. The context may have been destroyed before. */
+ * workspace. The context may have been destroyed before. Not while a stream of the
+ * device is captured: waiting spoils the capture, and the workspace is not freed. */
 TB_API void tb_cache_destroy(tb_cache *cache);
 /* Grow slots[i] by counts[i] tokens (counts NULL: one each): lengths go up and
  * the pages that are needed are taken, lowest free page first, in the order of

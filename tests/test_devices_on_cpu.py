@@ -39,3 +39,14 @@ def test_a_cache_may_outlive_its_context(lib):
     F.events(lib)
     lib.tb_cache_destroy(cache.h)
     assert F.events(lib) == ["synchronize 0", "free on 0"]
+
+
+def test_a_workspace_whose_calls_may_still_run_is_not_freed(lib, contexts):
+    """A device cannot be waited for while one of its streams is captured."""
+    lib.fake_set_device(0)
+    cache = F.HostCache(lib, contexts[0])
+    F.events(lib)
+    lib.fake_sync_result(900)
+    lib.tb_cache_destroy(cache.h)
+    lib.fake_sync_result(0)
+    assert F.events(lib) == ["synchronize 0"]

@@ -108,3 +108,27 @@ def test_results_given_by_the_caller_are_used_on_another_stream(ctx):
     got = attention(ctx, q, k, v, cu, cu, out=out, lse=lse, stream=side)
     side.synchronize()
     assert got[0] is out and got[1] is lse and torch.equal(out, want) and torch.equal(lse, wlse)
+
+
+@pytest.mark.parametrize("collected", [True, False])
+def test_a_cache_that_ends_during_a_capture_leaves_the_graph_whole(ctx, collected):
+    caches = [PagedCache.allocate(ctx, layers=1, num_pages=4, page_size=16, kv_heads=1, head_dim=64, dtype=torch.bfloat16,
+                                  max_seqs=2, max_pages=2) for _ in range(2)]
+    q, k, v = (torch.randn(50, h, 64, device="cuda").bfloat16() for h in (4, 2, 2))
+    cu = _offsets([50])
+    want, wlse = attention(ctx, q, k, v, cu, cu)
+    out, lse = torch.zeros_like(want), torch.zeros_like(wlse)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attention(ctx, q, k, v, cu, cu, out=out, lse=lse)
+        if collected:
+            del caches[0]
+        else:
+            caches[0].close()
+            assert caches[0].h is None
+    assert len(PagedCache._left) == 1
+    graph.replay()
+    ctx.synchronize()
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+    caches[-1].close()  # and with it the other one
+    assert not PagedCache._left

@@ -99,6 +99,7 @@ class PagedCache:
         b = L.CacheBuffers(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), refs.data_ptr())
         h = ctypes.c_void_p()
         self.h = None
+        self._destroy_left()
         with torch.cuda.device(k_pages.device):
             L.check(L.load().tb_cache_create(ctx.h, ctypes.byref(d), ctypes.byref(b), ctypes.byref(h)))
         self.h = h
@@ -113,10 +114,21 @@ class PagedCache:
         return cls(ctx, *pages, table, torch.zeros(max_seqs, dtype=torch.int32, device=dev),
                    torch.zeros(num_pages, dtype=torch.int32, device=dev))
 
+    _left = []  # handles of caches that were closed during a capture
+
     def close(self):
+        """Frees the workspace, after the device's work. That waiting would spoil a graph that the current stream is
+        capturing, so a cache that is closed (or collected) then is destroyed with the next one made or closed."""
         if self.h:
-            L.load().tb_cache_destroy(self.h)
+            self._left.append(self.h)
             self.h = None
+            self._destroy_left()
+
+    @classmethod
+    def _destroy_left(cls):
+        if cls._left and not torch.cuda.is_current_stream_capturing():
+            while cls._left:
+                L.load().tb_cache_destroy(cls._left.pop())
 
     def __del__(self):
         try:

@@ -631,8 +631,9 @@ TB_API void tb_cache_destroy(tb_cache* c) {
         int current = c->device;
         cudaGetDevice(&current);
         if (current != c->device) cudaSetDevice(c->device);
-        cudaDeviceSynchronize();  // the workspace may go to another cache at once: calls on any stream are through
-        cudaFreeAsync(c->blob, nullptr);
+        // The workspace may go to another cache at once: calls on any stream are through. (A device that could not be
+        // waited for, as while a stream of it is captured, keeps it.)
+        if (cudaDeviceSynchronize() == cudaSuccess) cudaFreeAsync(c->blob, nullptr);
         if (current != c->device) cudaSetDevice(current);
     }
     delete c;
