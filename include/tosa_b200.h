@@ -326,8 +326,9 @@ TB_API tb_status tb_max_pool2d(tb_context *ctx, const tb_pool2d_desc *desc, cons
  * Strides are elements from one token to the next and from one head to the next
  * (head_dim elements of a head are contiguous); strides are multiples of 8 and
  * pointers 16-byte aligned, so q, k and v may be parts of one projection's rows.
- * Asynchronous on `stream`; offsets out of range leave the sequence's rows
- * unwritten and are reported by the next tb_synchronize. */
+ * Asynchronous on `stream`; the context's device is the current one. Offsets out of
+ * range leave the sequence's rows unwritten and are reported by the next
+ * tb_synchronize. */
 typedef struct tb_attention_desc {
     int32_t dtype;            /* TB_DT_BF16 / TB_DT_FP16: q, k, v and out */
     int32_t batch;
@@ -354,8 +355,9 @@ TB_API tb_status tb_attention(tb_context *ctx, const tb_attention_desc *desc, co
  * A page that is not full belongs to one slot; full pages may be shared. A cache
  * starts with page_table -1, lengths 0 and refs 0. Slots, counts, offsets and
  * page ids passed below are DEVICE int32 arrays, so a step needs no host copy
- * and can be captured in a CUDA graph. Calls on one cache must not overlap on
- * the GPU (they share its state and workspace): use one stream, or order them.
+ * and can be captured in a CUDA graph. The context's device is current at a call.
+ * Calls on one cache must not overlap on the GPU (they share its state and
+ * workspace): use one stream, or order them.
  * Index arrays are checked on the device and what is wrong with them is reported
  * by the next tb_synchronize (TB_ERR_INVALID_ARGUMENT / TB_ERR_OUT_OF_PAGES):
  * a refused tb_cache_reserve, _fork or _free leaves the state unchanged; a write

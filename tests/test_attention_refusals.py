@@ -1,0 +1,32 @@
+"""What the torch form of attention and the cache refuses before anything reaches the library, without a GPU."""
+
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tosa_b200 import _lib as L  # noqa: E402
+from tosa_b200.attention import attention  # noqa: E402
+
+
+class Handle:
+    """A context with a handle that nothing may look behind."""
+
+    def __init__(self, device=0):
+        self.h, self.device = ctypes.c_void_p(1 << 12), device
+
+
+def _call(ctx=None, **kw):
+    # (a head_dim that the library refuses first thing, should the call get there)
+    t = dict(q=torch.zeros(4, 2, 24).half(), k=torch.zeros(6, 1, 24).half(), v=torch.zeros(6, 1, 24).half(),
+             cu_q=torch.tensor([0, 4], dtype=torch.int32), cu_k=torch.tensor([0, 6], dtype=torch.int32))
+    t.update(kw)
+    with pytest.raises(L.TbError) as e:
+        attention(ctx or Handle(), **t)
+    return e.value
+
+
+def test_tensors_that_are_not_on_a_gpu():
+    e = _call()
+    assert e.kind == "InvalidArgument" and "cpu" in str(e)

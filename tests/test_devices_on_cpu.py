@@ -1,8 +1,11 @@
 """Which device the library's host code waits for, allocates and launches on, without a GPU (fake_cuda.py)."""
 
+import ctypes
+
 import pytest
 
 from tests import fake_cuda as F
+from tosa_b200 import _lib as L
 
 
 @pytest.fixture(scope="module")
@@ -50,3 +53,31 @@ def test_a_workspace_whose_calls_may_still_run_is_not_freed(lib, contexts):
     lib.tb_cache_destroy(cache.h)
     lib.fake_sync_result(0)
     assert F.events(lib) == ["synchronize 0"]
+
+
+def test_calls_launch_on_the_contexts_device_only(lib, contexts):
+    lib.fake_set_device(0)
+    cache = F.HostCache(lib, contexts[0])
+    up = (ctypes.addressof(cache.k) + 255) & ~255
+    desc = L.AttentionDesc(dtype=L.DT_BF16, batch=1, q_heads=2, kv_heads=1, head_dim=64, causal=1, scale=0.125, total_q=4, total_k=4,
+                           q_token_stride=128, q_head_stride=64, k_token_stride=64, k_head_stride=64, v_token_stride=64,
+                           v_head_stride=64, out_token_stride=128, out_head_stride=64)
+    calls = [
+        lambda: lib.tb_attention(contexts[0], ctypes.byref(desc), up, up, up, up, up, up, None, None),
+        lambda: lib.tb_cache_reserve(cache.h, up, None, 1, None),
+        lambda: lib.tb_cache_write(cache.h, 0, up, up, 1, 1, up, 64, 64, up, 64, 64, None),
+        lambda: lib.tb_cache_attend(cache.h, 0, up, 1, 1, 0.125, up, 64, 64, up, 64, 64, None, None),
+        lambda: lib.tb_cache_fork(cache.h, up, up, 1, None),
+        lambda: lib.tb_cache_free(cache.h, up, 1, None),
+        lambda: lib.tb_cache_copy_pages(cache.h, up, up, 1, None),
+        lambda: lib.tb_cache_compact(cache.h, None, None, None),
+    ]
+    F.events(lib)
+    for i, call in enumerate(calls):
+        lib.fake_set_device(1)
+        assert call() == L.TB_ERR_INVALID_ARGUMENT, i
+        assert F.events(lib) == [], i
+        lib.fake_set_device(0)
+        assert call() == 0, (i, lib.tb_last_error())
+        assert set(F.events(lib)) == {"launch on 0"}, i
+    lib.tb_cache_destroy(cache.h)

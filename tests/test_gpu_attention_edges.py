@@ -132,3 +132,13 @@ def test_a_cache_that_ends_during_a_capture_leaves_the_graph_whole(ctx, collecte
     assert torch.equal(out, want) and torch.equal(lse, wlse)
     caches[-1].close()  # and with it the other one
     assert not PagedCache._left
+
+
+def test_tensors_on_another_device_than_the_contexts(ctx):
+    class Elsewhere:
+        h, device = ctx.h, ctx.device + 1
+
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(L.TbError) as e:
+        attention(Elsewhere(), q, q, q, _offsets([4]), _offsets([4]))
+    assert e.value.kind == "InvalidArgument"

@@ -899,6 +899,14 @@ tb_status attention_check(const char* op, int dtype, int q_heads, int kv_heads, 
     return TB_OK;
 }
 
+tb_status device_check(const char* op, const tb_context* ctx) {
+    int current = 0;
+    TB_CUDA(cudaGetDevice(&current));
+    if (current != ctx->device)
+        return fail(TB_ERR_INVALID_ARGUMENT, "%s: device %d is current, the context's is %d", op, current, ctx->device);
+    return TB_OK;
+}
+
 // [tokens][heads][head_dim] as {head_dim, heads, tokens}, boxes of some tokens by some heads by 64 elements.
 static tb_status tile_map(CUtensorMap* m, const tb_attention_desc* d, const void* p, int64_t heads, int64_t tokens,
                           int64_t token_stride, int64_t head_stride, int box_heads, int box_tokens) {
@@ -966,6 +974,7 @@ TB_API tb_status tb_attention(tb_context* ctx, const tb_attention_desc* d, const
     }
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (strides & 7))
         return fail(TB_ERR_INVALID_ARGUMENT, "attention: tensors must be 16-byte aligned with strides that are multiples of 8");
+    TB_TRY(device_check("attention", ctx));
     // without keys nothing is loaded; the maps are made of q's first row
     const bool keys = d->total_k > 0;
     CUtensorMap mq, mk, mv, mo;

@@ -62,5 +62,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // head_dim, heads, scale: the conditions that both attention operators share.
 tb_status attention_check(const char* op, int dtype, int q_heads, int kv_heads, int head_dim, float scale);
+// Kernels launch on the current device: it has to be the context's.
+tb_status device_check(const char* op, const tb_context* ctx);
 
 }  // namespace tb

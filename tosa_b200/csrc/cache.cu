@@ -17,6 +17,7 @@
 #include <initializer_list>
 #include <new>
 
+#include "attention.cuh"
 #include "cache.hpp"
 #include "ptx.cuh"
 #include "quant.cuh"
@@ -499,6 +500,7 @@ static tb_status cache_check(const tb_cache* c, const char* op, int n, bool dist
 // kernel's end; every kernel here waits for it before it reads anything).
 template <class... P, class... A>
 static tb_status launch(tb_context* ctx, void (*kernel)(P...), int grid, int block, cudaStream_t st, A... args) {
+    TB_TRY(device_check("cache", ctx));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(static_cast<unsigned>(block));
@@ -582,10 +584,7 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
         static_cast<long long>(d->max_pages) * d->page_size > (1ll << 30) ||
         d->layers > (1 << 16) || static_cast<long long>(d->layers) * d->kv_heads > (1ll << 29))
         return fail(TB_ERR_NOT_ACCELERATED, "cache: more than 2^30 rows or 2^16 layers");
-    int current = 0;
-    TB_CUDA(cudaGetDevice(&current));
-    if (current != ctx->device)
-        return fail(TB_ERR_INVALID_ARGUMENT, "cache: device %d is current, the context's is %d", current, ctx->device);
+    TB_TRY(device_check("cache", ctx));
     tb_cache* c = new (std::nothrow) tb_cache;
     if (!c) return fail(TB_ERR_INVALID_ARGUMENT, "cache: out of host memory");
     c->ctx = ctx;

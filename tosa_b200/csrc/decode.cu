@@ -698,6 +698,7 @@ TB_API tb_status tb_cache_attend(tb_cache* c, int32_t layer, const int32_t* slot
         return fail(TB_ERR_SHAPE_MISMATCH, "cache attend: negative stride");
     if (!aligned16(q) || !aligned16(out) || ((q_seq_stride | q_head_stride | out_seq_stride | out_head_stride) & 7))
         return fail(TB_ERR_INVALID_ARGUMENT, "cache attend: tensors must be 16-byte aligned with strides that are multiples of 8");
+    TB_TRY(device_check("cache attend", c->ctx));
     const int group = q_heads / d.kv_heads;
     DecodeArgs a{};
     a.q = static_cast<const uint16_t*>(q);

@@ -134,6 +134,17 @@ void* handle(const char* op, PyObject* o) {
     return p;
 }
 
+// A call's tensors (all on `device`) have to be on the context's device: elsewhere the kernel would use addresses that are not its own.
+void on_device_of(const char* op, PyObject* context, at::Device device) {
+    if (!device.is_cuda()) refuse(TB_ERR_INVALID_ARGUMENT, "%s: the tensors are on %s, not on a CUDA device", op, device.str().c_str());
+    PyObject* o = PyObject_GetAttrString(context, "device");
+    const long long own = o ? PyLong_AsLongLong(o) : -1;
+    Py_XDECREF(o);
+    if (PyErr_Occurred()) throw Refused{};
+    if (own != device.index())
+        refuse(TB_ERR_INVALID_ARGUMENT, "%s: the tensors are on %s, the context is on device %lld", op, device.str().c_str(), own);
+}
+
 // The stream of a call: the current one, or the given cudaStream_t.
 void* stream_of(PyObject* o, at::Device device) {
     if (o != Py_None) {
@@ -209,6 +220,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                   static_cast<int32_t>(hq.dim), causal, scale, hq.rows, hk.rows, hq.row_stride, hq.head_stride,
                                   hk.row_stride, hk.head_stride, hv.row_stride, hv.head_stride, ho.row_stride, ho.head_stride};
         auto* h = static_cast<tb_context*>(handle(op, a[0]));
+        on_device_of(op, a[0], device);
         void* st = stream_of(a[10], device);
         call(device, [&] { return tb_attention(h, &d, hq.p, hk.p, hv.p, cq.p, ck.p, ho.p,
                            static_cast<float*>(lse.data_ptr()), st); });
