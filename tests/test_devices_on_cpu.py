@@ -81,3 +81,19 @@ def test_calls_launch_on_the_contexts_device_only(lib, contexts):
         assert call() == 0, (i, lib.tb_last_error())
         assert set(F.events(lib)) == {"launch on 0"}, i
     lib.tb_cache_destroy(cache.h)
+
+
+def test_sizes_whose_indexes_pass_32_bits_are_refused(lib, contexts):
+    """A token's key of 2^31 vectors of 16 bytes, and a write of more slots than the search of their offsets can count."""
+    lib.fake_set_device(0)
+    cache = F.HostCache(lib, contexts[0])
+    w = ctypes.addressof(cache.words)
+    desc = L.CacheDesc(dtype=L.DT_BF16, layers=1, kv_heads=1 << 27, head_dim=128, page_size=8, num_pages=1, max_seqs=1, max_pages=1)
+    up = (ctypes.addressof(cache.k) + 255) & ~255
+    buffers, h = L.CacheBuffers(up, up, w, w, w), ctypes.c_void_p()
+    assert lib.tb_cache_create(contexts[0], ctypes.byref(desc), ctypes.byref(buffers), ctypes.byref(h)) == L.TB_ERR_NOT_ACCELERATED
+    assert not h.value
+    F.events(lib)
+    assert lib.tb_cache_write(cache.h, 0, up, up, 2**31 - 1, 1, up, 64, 64, up, 64, 64, None) == L.TB_ERR_NOT_ACCELERATED
+    assert F.events(lib) == []
+    lib.tb_cache_destroy(cache.h)

@@ -142,3 +142,34 @@ def test_tensors_on_another_device_than_the_contexts(ctx):
     with pytest.raises(L.TbError) as e:
         attention(Elsewhere(), q, q, q, _offsets([4]), _offsets([4]))
     assert e.value.kind == "InvalidArgument"
+
+
+def test_pages_of_more_than_32_bits_of_vectors(ctx):
+    """Pages of 2^27 tokens of 128, 2^31 vectors of 16 bytes each: a write to the second head of one, a copy of a whole
+    one. Keys and values are the same memory here, with the same contents, so that 64 GB are enough."""
+    tokens = 1 << 27
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 70 << 30:
+        pytest.skip("needs 70 GB of free memory")
+    memory = torch.empty(2 * tokens * 128, dtype=torch.bfloat16, device="cuda")
+    table, lengths, refs = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), _ints([tokens]), _ints([1])
+    pages = memory.view(1, 1, 2, tokens, 128)
+    c = PagedCache(ctx, pages, pages, table, lengths, refs)
+    pages[0, 0, :, -6:] = 0
+    x = torch.randn(5, 2, 128, device="cuda").bfloat16()
+    c.write(0, _ints([0]), _ints([0, 5]), x, x)
+    ctx.synchronize()
+    assert torch.equal(pages[0, 0, :, -5:], x.transpose(0, 1)) and (pages[0, 0, :, -6] == 0).all()
+    c.close()
+    pages = memory.view(1, 2, 1, tokens, 128)
+    c = PagedCache(ctx, pages, pages, table, lengths, _ints([1, 0]))
+    places = [0, 1, 12345677, tokens // 2, tokens - 2, tokens - 1]
+    x = torch.randn(len(places), 128, device="cuda").bfloat16()
+    for i, at in enumerate(places):
+        pages[0, 0, 0, at] = x[i]
+    c.copy_pages(_ints([0]), _ints([1]))
+    ctx.synchronize()
+    assert all(torch.equal(pages[0, 1, 0, at], x[i]) for i, at in enumerate(places))
+    c.close()
+    del pages, memory, c
+    torch.cuda.empty_cache()

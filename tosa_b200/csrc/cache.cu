@@ -385,10 +385,10 @@ __global__ void __launch_bounds__(256) cache_copy_kernel(CopyArgs a) {
             if (lane == 0) atomicOr(a.err, DEV_ERR_INDEX);
             continue;
         }
-        const int vecs = (a.rows ? __ldcg(a.rows + job) : a.page_size) * a.row_vecs;
+        const long long vecs = static_cast<long long>(a.rows ? __ldcg(a.rows + job) : a.page_size) * a.row_vecs;  // up to 2^34
         const uint4* from = base + ((static_cast<long long>(layer) * a.num_pages + src) * a.heads + head) * page_vecs;
         uint4* to = base + ((static_cast<long long>(layer) * a.num_pages + dst) * a.heads + head) * page_vecs;
-        for (int i = lane; i < vecs; i += 256) {
+        for (long long i = lane; i < vecs; i += 256) {
             uint4 x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -463,9 +463,9 @@ __global__ void __launch_bounds__(128) cache_write_kernel(WriteArgs a) {
     const bool is_v = w & 1;
     const uint4* from = is_v ? a.v + t * a.v_token : a.k + t * a.k_token;
     const long long hs = is_v ? a.v_head : a.k_head;
-    const int page_vecs = a.page_size * row_vecs;  // (a page of all heads is below 2^30 rows)
-    uint4* to = (is_v ? a.v_layer : a.k_layer) + static_cast<long long>(page) * a.heads * page_vecs + (pos % a.page_size) * row_vecs;
-    const int vecs = a.heads * row_vecs;
+    const long long page_vecs = static_cast<long long>(a.page_size) * row_vecs;  // of one head, up to 2^34
+    uint4* to = (is_v ? a.v_layer : a.k_layer) + page * a.heads * page_vecs + static_cast<long long>(pos % a.page_size) * row_vecs;
+    const int vecs = a.heads * row_vecs;  // at most 2^30
     for (int i0 = lane; i0 < vecs; i0 += 256) {
         uint4 x[8];
 #pragma unroll
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(128) cache_write_kernel(WriteArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int i = i0 + 32 * j, h = i / row_vecs;
-            if (i < vecs) to[static_cast<long long>(h) * page_vecs + (i - h * row_vecs)] = x[j];
+            if (i < vecs) to[h * page_vecs + (i - h * row_vecs)] = x[j];
         }
     }
 }
@@ -584,6 +584,9 @@ TB_API tb_status tb_cache_create(tb_context* ctx, const tb_cache_desc* d, const 
         static_cast<long long>(d->max_pages) * d->page_size > (1ll << 30) ||
         d->layers > (1 << 16) || static_cast<long long>(d->layers) * d->kv_heads > (1ll << 29))
         return fail(TB_ERR_NOT_ACCELERATED, "cache: more than 2^30 rows or 2^16 layers");
+    // a token's key is written with 32-bit indexes of 16-byte vectors
+    if (static_cast<long long>(d->kv_heads) * (d->head_dim / 8) > (1ll << 30))
+        return fail(TB_ERR_NOT_ACCELERATED, "cache: more than 2^33 elements in a token's key");
     TB_TRY(device_check("cache", ctx));
     tb_cache* c = new (std::nothrow) tb_cache;
     if (!c) return fail(TB_ERR_INVALID_ARGUMENT, "cache: out of host memory");
@@ -698,6 +701,7 @@ TB_API tb_status tb_cache_write(tb_cache* c, int32_t layer, const int32_t* slots
     if (layer < 0 || layer >= c->d.layers)
         return fail(TB_ERR_SHAPE_MISMATCH, "cache write: layer %d of %d", layer, c->d.layers);
     if (total < 0 || total > (1ll << 30)) return fail(TB_ERR_SHAPE_MISMATCH, "cache write: %lld rows", (long long)total);
+    if (n > (1 << 30)) return fail(TB_ERR_NOT_ACCELERATED, "cache write: more than 2^30 slots");  // (32-bit search)
     if (total > 0 && n == 0) return fail(TB_ERR_SHAPE_MISMATCH, "cache write: rows without a slot");
     if (total == 0) return TB_OK;
     if (!k || !v) return fail(TB_ERR_INVALID_ARGUMENT, "cache write: null pointer");
