@@ -97,3 +97,21 @@ def test_sizes_whose_indexes_pass_32_bits_are_refused(lib, contexts):
     assert lib.tb_cache_write(cache.h, 0, up, up, 2**31 - 1, 1, up, 64, 64, up, 64, 64, None) == L.TB_ERR_NOT_ACCELERATED
     assert F.events(lib) == []
     lib.tb_cache_destroy(cache.h)
+
+
+def test_every_device_gets_the_shared_memory_that_a_kernel_needs(lib, contexts):
+    """The limit of a function's dynamic shared memory is each device's own: one process may have contexts on several."""
+    for device, ctx in enumerate(contexts):
+        lib.fake_set_device(device)
+        cache = F.HostCache(lib, ctx)
+        up = (ctypes.addressof(cache.k) + 255) & ~255
+        heads = L.AttentionDesc(dtype=L.DT_FP16, batch=1, q_heads=2, kv_heads=1, head_dim=128, causal=1, scale=0.125, total_q=4,
+                                total_k=4, q_token_stride=256, q_head_stride=128, k_token_stride=128, k_head_stride=128,
+                                v_token_stride=128, v_head_stride=128, out_token_stride=256, out_head_stride=128)
+        product = L.MatmulDesc(n=1, h=64, c=64, w=64, a_dtype=L.DT_BF16, b_dtype=L.DT_BF16, out_dtype=L.DT_FP32)
+        F.events(lib)
+        assert lib.tb_attention(ctx, ctypes.byref(heads), up, up, up, up, up, up, None, None) == 0, (device, lib.tb_last_error())
+        assert lib.tb_cache_attend(cache.h, 0, up, 1, 2, 0.125, up, 128, 64, up, 128, 64, None, None) == 0, (device, lib.tb_last_error())
+        assert lib.tb_matmul_t(ctx, product, 1, None, up, up, up, None) == 0, (device, lib.tb_last_error())
+        assert set(F.events(lib)) == {f"launch on {device}"}
+        lib.tb_cache_destroy(cache.h)

@@ -924,16 +924,16 @@ static tb_status launch_prompt(tb_context* ctx, const CUtensorMap& q, const CUte
                                const CUtensorMap& o, const PromptArgs& a, long long grid, cudaStream_t st) {
     auto* kernel = prompt_kernel<BF16, DCH>;
     constexpr int kSmem = PromptCfg<DCH>::kTiles + static_cast<int>(sizeof(PromptShared));
-    static bool ready = false;  // the attribute is per function and process-wide
-    if (!ready) {
+    static OncePerDevice once;
+    TB_TRY(once([&]() -> tb_status {
         // the warpgroups re-split the registers of the launch (setmaxnreg), which needs all of them
         cudaFuncAttributes fa;
         TB_CUDA(cudaFuncGetAttributes(&fa, kernel));
         if (fa.numRegs < kLaunchRegs)
             return fail(TB_ERR_CUDA, "attention built with %d registers a thread; its register split needs %d", fa.numRegs, kLaunchRegs);
         TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-        ready = true;
-    }
+        return TB_OK;
+    }));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(kThreads);

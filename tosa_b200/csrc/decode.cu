@@ -649,11 +649,11 @@ tb_status decode_create(tb_cache* c) {
 template <bool BF16, int DCH, int NT>
 static tb_status launch_decode(tb_cache* c, int layer, const DecodeArgs& a, cudaStream_t st) {
     auto* kernel = decode_kernel<BF16, DCH, NT>;
-    static bool ready = false;  // the attribute is per function and process-wide
-    if (!ready) {
+    static OncePerDevice once;
+    TB_TRY(once([&]() -> tb_status {
         TB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<DCH>::kSmem));
-        ready = true;
-    }
+        return TB_OK;
+    }));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(c->decode_ctas));
     cfg.blockDim = dim3(kDecodeThreads);

@@ -36,8 +36,8 @@ inline FastDiv make_fastdiv(int d) {
 template <class Cfg, int EK, int EF = 0>
 tb_status launch_gemm(tb_context* ctx, const CUtensorMap& tmA, const CUtensorMap& tmB, GemmParams p,
                       cudaStream_t stream) {
-    static bool attr_set = false;  // the attribute is per function and process-wide
-    if (!attr_set) {
+    static OncePerDevice once;
+    TB_TRY(once([&]() -> tb_status {
         // The kernel's warpgroups re-split the registers it was launched with (setmaxnreg); that
         // needs the full launch allocation, or the epilogue warps would wait for registers forever.
         cudaFuncAttributes fa;
@@ -47,8 +47,8 @@ tb_status launch_gemm(tb_context* ctx, const CUtensorMap& tmA, const CUtensorMap
                         fa.numRegs, kLaunchRegs);
         TB_CUDA(cudaFuncSetAttribute(tc_gemm_kernel<Cfg, EK, EF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      Cfg::SMEM_BYTES));
-        attr_set = true;
-    }
+        return TB_OK;
+    }));
     p.m_tiles = (p.M + Cfg::BM - 1) / Cfg::BM;
     p.n_tiles = (p.N + Cfg::kBN - 1) / Cfg::kBN;
     p.total_tiles = p.batch * p.m_tiles * p.n_tiles;

@@ -474,12 +474,12 @@ tb_status launch_residual(tb_context* ctx, const void* a, int a_dt, int a_uns, i
         // whose third table load per SM cost more than the extra threads gained.
         const int grid = static_cast<int>(std::max<long long>(
             1, std::min<long long>((n16 + 2047) / 2048, 2ll * ctx->num_sms)));
-        static bool attr_set = false;
-        if (!attr_set) {
+        static OncePerDevice once;
+        TB_TRY(once([&]() -> tb_status {
             TB_CUDA(cudaFuncSetAttribute(residual_table_i8, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kResidTableBytes));
-            attr_set = true;
-        }
+            return TB_OK;
+        }));
         residual_table_i8<<<grid, 1024, kResidTableBytes, st>>>(static_cast<const uint4*>(a),
                                                                static_cast<const uint4*>(b),
                                                                reinterpret_cast<const uint4*>(fast.d_table), n16,
@@ -499,12 +499,12 @@ tb_status launch_residual(tb_context* ctx, const void* a, int a_dt, int a_uns, i
         auto O = static_cast<uint4*>(out);
 #define TB_RESID(PC, DBL, SMALL)                                                                                  \
     do {                                                                                                     \
-        static bool attr_set = false;                                                                        \
-        if (!attr_set) {                                                                                     \
+        static OncePerDevice once;                                                                           \
+        TB_TRY(once([&]() -> tb_status {                                                                     \
             TB_CUDA(cudaFuncSetAttribute(residual_fast_i8<PC, DBL, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
                                          kResidLutBytes));                                                   \
-            attr_set = true;                                                                                 \
-        }                                                                                                    \
+            return TB_OK;                                                                                    \
+        }));                                                                                                 \
         residual_fast_i8<PC, DBL, SMALL><<<grid, 256, kResidLutBytes, st>>>(A, B, fast, ro.fq_m, ro.fq_sh, ro.fq_hz, \
                                                                             ro.lo, ro.hi, add_zp, n16, channels, O); \
     } while (0)

@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -55,6 +56,24 @@ tb_status fail(tb_status st, const char* fmt, ...);
         tb_status s_ = (expr);               \
         if (s_ != TB_OK) return s_;          \
     } while (0)
+
+// Attributes of a function (its limit of dynamic shared memory) belong to each device's copy of it: set() runs when a
+// launch first finds the current device. Threads that find it at the same time may each run it, to the same end.
+class OncePerDevice {
+    std::atomic<uint64_t> done_{0};  // a bit a device; from the 64th on set() runs every time
+
+  public:
+    template <class F>
+    tb_status operator()(F set) {
+        int d = 0;
+        TB_CUDA(cudaGetDevice(&d));
+        const uint64_t bit = d < 64 ? 1ull << d : 0;
+        if (done_.load(std::memory_order_acquire) & bit) return TB_OK;
+        TB_TRY(set());
+        done_.fetch_or(bit, std::memory_order_release);
+        return TB_OK;
+    }
+};
 
 // Driver entry points fetched through the runtime (no libcuda link).
 tb_status encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
