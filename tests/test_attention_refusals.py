@@ -30,3 +30,14 @@ def _call(ctx=None, **kw):
 def test_tensors_that_are_not_on_a_gpu():
     e = _call()
     assert e.kind == "InvalidArgument" and "cpu" in str(e)
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "out"])
+def test_a_gradient_that_would_be_lost(name):
+    """There is no backward pass: results would come without a gradient, silently."""
+    rows = 6 if name in "kv" else 4
+    t = {name: torch.zeros(rows, 1 if name in "kv" else 2, 24).half().requires_grad_()}
+    e = _call(**t)
+    assert e.kind == "InvalidArgument" and "gradient" in str(e) and f": {name} " in str(e)
+    with torch.no_grad():
+        assert "gradient" not in str(_call(**t))

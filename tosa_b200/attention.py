@@ -14,7 +14,8 @@ The Python form of the header's tb_attention and tb_cache_* entry points:
 Index tensors are int32 on the device. Calls are asynchronous on the current
 stream, or on `stream`; what a kernel finds wrong in an index tensor is raised
 by the next ctx.synchronize(). Everything that can be seen on the host (types,
-shapes, strides, alignment) raises TbError at the call.
+shapes, strides, alignment) raises TbError at the call. There is no backward
+pass: a tensor that requires a gradient is refused outside torch.no_grad().
 """
 
 from __future__ import annotations

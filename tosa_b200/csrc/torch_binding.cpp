@@ -8,6 +8,7 @@
 
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -83,6 +84,8 @@ Heads heads(const char* op, const char* name, const at::Tensor& t, at::ScalarTyp
         refuse(TB_ERR_INVALID_ARGUMENT, "%s: %s is on %s, not on %s", op, name, t.device().str().c_str(), device.str().c_str());
     if (t.dim() != 3 || (rows >= 0 && t.size(0) != rows) || (n >= 0 && t.size(1) != n) || (dim >= 0 && t.size(2) != dim))
         refuse(TB_ERR_SHAPE_MISMATCH, "%s: %s has shape %s", op, name, shape_of(t).c_str());
+    if (t.requires_grad() && c10::GradMode::is_enabled())
+        refuse(TB_ERR_INVALID_ARGUMENT, "%s: %s requires a gradient, and there is none (torch.no_grad() or %s.detach())", op, name, name);
     if (t.stride(2) != 1) refuse(TB_ERR_SHAPE_MISMATCH, "%s: the last dimension of %s must be contiguous", op, name);
     // the stride of a dimension of one element says nothing
     return Heads{t.data_ptr(), t.size(0), t.size(1), t.size(2), t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2),
