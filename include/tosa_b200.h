@@ -355,7 +355,8 @@ TB_API tb_status tb_attention(tb_context *ctx, const tb_attention_desc *desc, co
  * A page that is not full belongs to one slot; full pages may be shared. A cache
  * starts with page_table -1, lengths 0 and refs 0. Slots, counts, offsets and
  * page ids passed below are DEVICE int32 arrays, so a step needs no host copy
- * and can be captured in a CUDA graph. The context's device is current at a call.
+ * and can be captured in a CUDA graph. The context's device is current at a call,
+ * and the context lives for as long as calls are made.
  * Calls on one cache must not overlap on the GPU (they share its state and
  * workspace): use one stream, or order them.
  * Index arrays are checked on the device and what is wrong with them is reported

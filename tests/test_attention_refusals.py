@@ -7,7 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from tosa_b200 import _lib as L  # noqa: E402
-from tosa_b200.attention import attention  # noqa: E402
+from tosa_b200.attention import PagedCache, attention  # noqa: E402
 
 
 class Handle:
@@ -41,3 +41,21 @@ def test_a_gradient_that_would_be_lost(name):
     assert e.kind == "InvalidArgument" and "gradient" in str(e) and f": {name} " in str(e)
     with torch.no_grad():
         assert "gradient" not in str(_call(**t))
+
+
+@pytest.mark.parametrize("op", ["reserve", "write", "attend", "fork", "free", "copy_pages"])
+def test_a_cache_whose_context_is_closed(op):
+    """The library's cache points into its context. (What stands for one here is zeros, and the calls have nothing to do.)"""
+    zeros = ctypes.create_string_buffer(1 << 12)
+    c = PagedCache.__new__(PagedCache)
+    c.h, c.ctx = ctypes.c_void_p(ctypes.addressof(zeros)), Handle()
+    c.ctx.h = None
+    c.k_pages = torch.zeros(1, 4, 1, 8, 64).half()
+    none, x = torch.zeros(0, dtype=torch.int32), torch.zeros(0, 1, 64).half()
+    args = dict(write=(0, none, torch.zeros(1, dtype=torch.int32), x, x), attend=(0, none, x), fork=(none, none), copy_pages=(none, none))
+    try:
+        with pytest.raises(L.TbError) as e:
+            getattr(c, op)(*args.get(op, (none,)))
+        assert e.value.kind == "InvalidArgument" and "closed" in str(e.value)
+    finally:
+        c.h = None

@@ -137,6 +137,20 @@ void* handle(const char* op, PyObject* o) {
     return p;
 }
 
+// A cache's handle, which points into its context.
+tb_cache* cache_handle(const char* op, PyObject* o) {
+    PyObject* context = PyObject_GetAttrString(o, "ctx");
+    if (!context) throw Refused{};
+    PyObject* h = PyObject_GetAttrString(context, "h");
+    const bool closed = h == Py_None;
+    const bool missing = h == nullptr;
+    Py_XDECREF(h);
+    Py_DECREF(context);
+    if (missing) throw Refused{};
+    if (closed) refuse(TB_ERR_INVALID_ARGUMENT, "%s: the cache's context is closed", op);
+    return static_cast<tb_cache*>(handle(op, o));
+}
+
 // A call's tensors (all on `device`) have to be on the context's device: elsewhere the kernel would use addresses that are not its own.
 void on_device_of(const char* op, PyObject* context, at::Device device) {
     if (!device.is_cuda()) refuse(TB_ERR_INVALID_ARGUMENT, "%s: the tensors are on %s, not on a CUDA device", op, device.str().c_str());
@@ -242,7 +256,7 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Index offsets = index(op, "offsets", a[4], device, static_cast<int64_t>(slots.n) + 1);
         const Heads k = heads(op, "k", tensor(op, "k", a[5]), pages.scalar_type(), device, -1, pages.size(2), pages.size(4));
         const Heads v = heads(op, "v", tensor(op, "v", a[6]), pages.scalar_type(), device, k.rows, pages.size(2), pages.size(4));
-        auto* h = static_cast<tb_cache*>(handle(op, a[0]));
+        tb_cache* h = cache_handle(op, a[0]);
         void* st = stream_of(a[7], device);
         call(device, [&] { return tb_cache_write(h, layer, slots.p, offsets.p, slots.n, k.rows, k.p, k.row_stride,
                              k.head_stride, v.p, v.row_stride, v.head_stride, st); });
@@ -266,7 +280,7 @@ PyObject* cache_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                                : tensor(op, "out", a[6]);
         const Heads ho = heads(op, "out", out, type, device, q.rows, q.heads, q.dim);
         const at::Tensor lse = sums(op, a[7], q.rows, q.heads, device);
-        auto* h = static_cast<tb_cache*>(handle(op, a[0]));
+        tb_cache* h = cache_handle(op, a[0]);
         void* st = stream_of(a[8], device);
         call(device, [&] { return tb_cache_attend(h, layer, slots.p, slots.n, static_cast<int32_t>(q.heads), scale,
                               q.p, q.row_stride, q.head_stride, ho.p, ho.row_stride, ho.head_stride,
@@ -282,7 +296,7 @@ PyObject* cache_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Device device = tensor(op, "k_pages", a[1]).device();
         const Index slots = index(op, "slots", a[2], device);
         const int32_t* counts = a[3] == Py_None ? nullptr : index(op, "counts", a[3], device, slots.n).p;
-        auto* h = static_cast<tb_cache*>(handle(op, a[0]));
+        tb_cache* h = cache_handle(op, a[0]);
         void* st = stream_of(a[4], device);
         call(device, [&] { return tb_cache_reserve(h, slots.p, counts, slots.n, st); });
         return none();
@@ -295,7 +309,7 @@ PyObject* cache_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const char* op = "cache free";
         const at::Device device = tensor(op, "k_pages", a[1]).device();
         const Index slots = index(op, "slots", a[2], device);
-        auto* h = static_cast<tb_cache*>(handle(op, a[0]));
+        tb_cache* h = cache_handle(op, a[0]);
         void* st = stream_of(a[3], device);
         call(device, [&] { return tb_cache_free(h, slots.p, slots.n, st); });
         return none();
@@ -309,7 +323,7 @@ PyObject* cache_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Device device = tensor(op, "k_pages", a[1]).device();
         const Index parents = index(op, "parents", a[2], device);
         const Index children = index(op, "children", a[3], device, parents.n);
-        auto* h = static_cast<tb_cache*>(handle(op, a[0]));
+        tb_cache* h = cache_handle(op, a[0]);
         void* st = stream_of(a[4], device);
         call(device, [&] { return tb_cache_fork(h, parents.p, children.p, parents.n, st); });
         return none();
@@ -323,7 +337,7 @@ PyObject* cache_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Device device = tensor(op, "k_pages", a[1]).device();
         const Index src = index(op, "src", a[2], device);
         const Index dst = index(op, "dst", a[3], device, src.n);
-        auto* h = static_cast<tb_cache*>(handle(op, a[0]));
+        tb_cache* h = cache_handle(op, a[0]);
         void* st = stream_of(a[4], device);
         call(device, [&] { return tb_cache_copy_pages(h, src.p, dst.p, src.n, st); });
         return none();
@@ -344,7 +358,7 @@ PyObject* cache_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 refuse(TB_ERR_SHAPE_MISMATCH, "%s: %s must be like the cache's own", op, names[i]);
             to[i] = static_cast<int32_t*>(t.data_ptr());
         }
-        auto* h = static_cast<tb_cache*>(handle(op, a[0]));
+        tb_cache* h = cache_handle(op, a[0]);
         void* st = stream_of(a[5], device);
         call(device, [&] { return tb_cache_compact(h, to[0], to[1], st); });
         return none();
