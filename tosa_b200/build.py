@@ -6,7 +6,8 @@ Each translation unit under csrc/ is compiled in parallel into _build/ and the
 objects are linked into tosa_b200/libtosa_b200.so (CUDA runtime linked
 statically; driver entry points are resolved at run time).
 csrc/torch_binding.cpp is compiled with the host compiler against the
-installed torch into tosa_b200/_torch_binding.so, which loads that library.
+installed torch into tosa_b200/_torch_binding.so, which loads that library;
+without torch the library is built alone.
 """
 
 from __future__ import annotations
@@ -44,7 +45,11 @@ def _start_binding(force, verbose):
         return None
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        print("torch is not installed: built without the torch binding (tosa_b200/attention.py needs it)", file=sys.stderr)
+        return None
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(NVCC))
     obj = os.path.join(BUILD, "torch_binding.cpp.o")
