@@ -173,3 +173,29 @@ def test_pages_of_more_than_32_bits_of_vectors(ctx):
     c.close()
     del pages, memory, c
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("heads,d", [(2, 128), (1, 64)])
+def test_attend_under_a_bound_of_zero_is_right_or_says_that_a_wait_ran_out(heads, d):
+    """Its waits are for copies of some microseconds, which the first look at a barrier may outlast: a wait that gives up
+    cannot be brought about at will. Where one does, the kernel goes through its units without data, its loads land and
+    the next synchronize reports it. The call after that is right either way."""
+    lib, ctx = L.load(), L.Context(0)
+    c, slots, q, k, v = _filled(ctx, [5000, 70, 9000], heads, d)
+    want, wlse = c.attend(0, slots, q)
+    ctx.synchronize()
+    for _ in range(20):
+        L.check(lib.tb_context_set_wait_timeout_ms(ctx.h, 0.0))
+        out, lse = c.attend(0, slots, q)
+        try:
+            ctx.synchronize()
+        except L.TbError as e:
+            assert e.kind == "Timeout"
+        else:
+            assert torch.equal(out, want) and torch.equal(lse, wlse)
+        L.check(lib.tb_context_set_wait_timeout_ms(ctx.h, 2000.0))
+        out, lse = c.attend(0, slots, q)
+        ctx.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, wlse)
+    c.close()
+    ctx.close()

@@ -250,6 +250,12 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
         // ---------------------------------------------------------------- loads
         const int pieces = kTokens / a.box;  // at most 8
         const long long drain = limit > kDecodeDrain ? limit : kDecodeDrain;
+        // A place in the ring or of the query rows is free. Warps 0-3 release places without their data when they have given
+        // up; the abort flag, raised before, then tells that a copy may still be on its way there, and that its barrier
+        // must not be armed once more.
+        auto free_place = [&](uint64_t* bar, uint32_t ph) {
+            return __all_sync(0xffffffffu, mbar_wait_bounded(bar, ph, abort_flag, limit) && *abort_flag == 0) != 0;
+        };
         uint32_t it = 0, seg = 0;
         bool ok = true;
         while (ok && walk.next(a)) {
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
             };
             int page = lookup(walk.t0);
             const int qs = seg & (q_slots - 1);
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.q_empty[qs], ((seg / q_slots) & 1) ^ 1, abort_flag, limit));
+            ok = free_place(&sh.q_empty[qs], ((seg / q_slots) & 1) ^ 1);
             if (!ok) break;
             const uint32_t row_bytes = a.head_dim * 2;
             if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[qs], rows * row_bytes);
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
             ++seg;
             for (int t = walk.t0; t < walk.t1; ++t, ++it) {
                 const int s = it % S;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.empty[s], ((it / S) & 1) ^ 1, abort_flag, limit));
+                ok = free_place(&sh.empty[s], ((it / S) & 1) ^ 1);
                 if (!ok) break;
                 const int tok = t * kTokens + lane * a.box;
                 const bool mine = lane < pieces && tok < walk.len;
