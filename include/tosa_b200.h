@@ -318,7 +318,9 @@ TB_API tb_status tb_max_pool2d(tb_context *ctx, const tb_pool2d_desc *desc, cons
  *   out[i,h] = sum_j w_j v[j] / sum_j w_j,  w_j = exp(scale * q[i,h].k[j]),
  *   lse[h][i] = log sum_j w_j  (FP32, [q_heads][total_q]; lse may be NULL),
  * over every j, or with `causal` over j <= i + lk - lq (the last row sees every
- * key). A row that sees no key gives out 0 and lse -inf. Keys that a row does
+ * key). A row that sees no key gives out 0 and lse -inf. One that sees keys but
+ * whose every score is -inf is 0 divided by 0: out NaN, lse -inf. A score of NaN or
+ * +inf that it sees makes its out and lse NaN. Keys that a row does
  * not see have no part in it, whatever they hold. Products are of f16 / bf16
  * operands with FP32 sums; the weights are rounded to the operands' type for
  * the second product and are summed in FP32 before that rounding.

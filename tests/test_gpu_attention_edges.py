@@ -199,3 +199,25 @@ def test_attend_under_a_bound_of_zero_is_right_or_says_that_a_wait_ran_out(heads
         assert torch.equal(out, want) and torch.equal(lse, wlse)
     c.close()
     ctx.close()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,at", [(40, 3), (40, 39), (5000, 0), (5000, 31), (5000, 64), (5000, 4999)])
+def test_infinite_scores_of_one_new_token_and_of_a_prompts_row(ctx, n, at, d):
+    """Every score -inf: 0 divided by 0, and the logarithm of 0. One of +inf, anywhere: infinity by infinity. In one CTA and
+    in several, in the first 32 keys and after them."""
+    lens = [n, n, 50]
+    c, slots, q, k, v = _filled(ctx, lens, 1, d)
+    q[:2], k[:2 * n] = q[:2].abs(), k[:2 * n].abs()
+    want, wlse = c.attend(0, slots, q)
+    k[:n, :, 5] = -math.inf
+    k[n + at, :, 5] = math.inf
+    c.write(0, slots, _offsets(lens), k, v)
+    out, lse = c.attend(0, slots, q)
+    rows, rlse = attention(ctx, q, k, v, _offsets([1, 1, 1]), _offsets(lens))
+    ctx.synchronize()
+    for o, s in ((out, lse), (rows, rlse.T)):
+        assert torch.isnan(o[0]).all() and (s[0] == -math.inf).all()
+        assert torch.isnan(o[1]).all() and torch.isnan(s[1]).all()
+        assert torch.isfinite(o[2]).all() and torch.isfinite(s[2]).all()
+    assert torch.equal(out[2], want[2]) and torch.equal(lse[2], wlse[2])
