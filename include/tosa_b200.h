@@ -330,7 +330,7 @@ TB_API tb_status tb_max_pool2d(tb_context *ctx, const tb_pool2d_desc *desc, cons
  * pointers 16-byte aligned, so q, k and v may be parts of one projection's rows.
  * Asynchronous on `stream`; the context's device is the current one. Offsets out of
  * range leave the sequence's rows unwritten and are reported by the next
- * tb_synchronize. */
+ * tb_synchronize; rows of q that lie in no sequence are not written either. */
 typedef struct tb_attention_desc {
     int32_t dtype;            /* TB_DT_BF16 / TB_DT_FP16: q, k, v and out */
     int32_t batch;

@@ -8,7 +8,8 @@
 // everything before it changes anything, so a refused call leaves the state as it
 // was. Such a block's time is its chain of dependent accesses, some 0.7 us each: values that
 // only the end of a call changes are read through L1, eight lanes take a slot's pages so that 128 slots
-// are looked at together, and checks share a barrier (fork of 64 children, with its copies, 31.9 -> 25.7 us).
+// are looked at together, and checks share a barrier (fork of 64 children, with its copies, 31.9 -> 25.9 us; 26.2 since
+// copies count their vectors in 64 bits).
 // Moving page contents is a second, grid-wide kernel that reads the list the first one left; it is bound by
 // memory bandwidth.
 #include <cuda_runtime.h>

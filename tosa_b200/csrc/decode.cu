@@ -1,9 +1,10 @@
 // Attention of one new token a sequence over the paged cache.
 //
-// The formula is attention.cu's with one row a sequence. Every key and value is read once and used
-// for the group's query heads only, so the kernel is bound by memory bandwidth: its work is cut so that
-// every SM streams the same amount, and the arithmetic only has to keep up. Keys and dimensions take
-// the long side of mma.sync's 16 x 8 x 16 and the query rows the short one, so at most 7 rows are padding.
+// The formula is attention.cu's with one row a sequence. For groups of up to 16 query heads a key head every key and
+// value is read once and used for that group only, so the kernel is bound by memory bandwidth: its work is cut so that
+// every SM streams the same amount, and the arithmetic only has to keep up. Keys and dimensions take the long side of
+// mma.sync's 16 x 8 x 16 and the query rows the short one: a unit's rows are padded to 8, or to 16 in groups above 8.
+// (A group above 16 is several units, each of which asks for its keys again.)
 //
 // Cut: a unit is one sequence, key head and at most 8 (for groups above 8: 16) of its query heads; its keys
 // come in tiles of 64 tokens. The tiles of all units in a row are divided evenly over the CTAs (two on each
